@@ -261,6 +261,192 @@ int tilemix_quantize_qk_strided(const uint16_t* Q, const uint16_t* K, int8_t* Q8
                                 int d, int64_t q_head_stride, int64_t k_head_stride,
                                 int64_t q_row_stride, int64_t k_row_stride, void* stream);
 
+/* ------------------------------------------------------------------------
+ * Serving: prompts of different lengths in one call, and a paged key/value
+ * cache held in 4 bits (no reference counterpart: the reference has one dense
+ * head per call).
+ *
+ * Common to these entry points: tensors are [tokens][heads][d] of fp16 or bf16
+ * values (`dtype`: TILEMIX_DTYPE_F16 / _BF16; inputs and outputs alike), d a
+ * multiple of 8 up to 128, head h of token t at t * row_stride + h * head_stride
+ * elements (0: dense, heads * d and d). Strides are multiples of 8 elements (4
+ * for O) and addresses of 16 bytes (8 for O); heads must not overlap.
+ * kv_heads divides q_heads, and query head h reads key head h / (q_heads /
+ * kv_heads). Lengths, tables and slots are read on the device when the kernel
+ * runs, so that a captured call takes their values at replay; whatever they
+ * hold, nothing outside the tensors, tables and pages named here is read or
+ * written. Errors: null pointer, bad size, stride, alignment or dtype, d not a
+ * multiple of 8 -> InvalidValue; d > 128 -> NotSupported. No entry point
+ * allocates or synchronises. */
+
+/* O = softmax(score_scale * Q K^T) V of `batch` packed sequences. Sequence b has
+ * the query rows q_starts[b] .. q_starts[b + 1] - 1 and the keys k_starts[b] ..
+ * k_starts[b + 1] - 1 ([batch + 1] device arrays; k_starts NULL: q_starts), either
+ * possibly none. causal: rows are aligned at the end of their keys - row i of Lq
+ * sees keys 0 .. i + Lk - Lq of Lk, all of its prompt's keys so far. A row that
+ * sees no key becomes 0; rows of O outside every sequence are left as they were.
+ * Keys and values that a row does not see do not reach it, whatever they hold.
+ * Starts are clamped to 0 .. q_tokens / k_tokens; where they decrease, the
+ * sequence is empty. q_tokens or batch 0: nothing to do. k_row_stride and
+ * v_row_stride up to 2^24 elements (more: NotSupported). */
+typedef struct TileMixPackedAttentionArgs {
+    const uint16_t* Q;
+    const uint16_t* K;
+    const uint16_t* V;
+    uint16_t* O;
+    const int32_t* q_starts;
+    const int32_t* k_starts;
+    int batch;
+    int q_tokens; /* rows of Q and O */
+    int k_tokens; /* rows of K and V */
+    int q_heads;
+    int kv_heads;
+    int d;
+    int dtype;
+    int causal;
+    float score_scale;
+    int64_t q_row_stride;
+    int64_t k_row_stride;
+    int64_t v_row_stride;
+    int64_t o_row_stride;
+    int64_t q_head_stride;
+    int64_t k_head_stride;
+    int64_t v_head_stride;
+    int64_t o_head_stride;
+} TileMixPackedAttentionArgs;
+
+int tilemix_attention_packed(const TileMixPackedAttentionArgs* args, void* stream);
+
+/* The cache: `pages` pages of page_size tokens (a multiple of 32) for kv_heads
+ * key heads, [pages][kv_heads][page_size / 32] blocks of tilemix_cache4_block_bytes
+ * (d) bytes, 16-byte aligned; tilemix_cache4_bytes of them in all. A slot is
+ * page * page_size + place in the page. Every 64 features of one token and head
+ * (the last group possibly fewer) share a scale and a minimum, bf16 both, beside
+ * their 4-bit codes: 4.5 bits a value for d of 64 or 128 (rows of other d take
+ * the room of the next of these two). x is held as minimum + scale * code with
+ *   minimum = bf16(least x), scale = bf16((largest x - minimum) / 15),
+ *   code = clamp(round_half_even((x - minimum) / scale), 0, 15),
+ * 0 where scale is below 2^-100; a group with an infinite or NaN value (or
+ * a range past fp32's) is held as NaN. Order inside a block, with B = ceil(d / 64):
+ *   key codes: 8 B words a token; features 64 m + 16 g + 8 w + e in word
+ *     2 B g + 2 m + w, feature e (0 .. 7) at bits 4 (e / 2) + 16 (e % 2);
+ *   value codes: [16 B][32 places] of 16 bits, features 4 q + f at bits 4 f of row q;
+ *   key, then value parameters: [B][32 places] of (scale, minimum);
+ * token t (0 .. 31) has the place 8 ((t % 16) / 4) + 4 (t / 16) + t % 4. Sizes
+ * that are not valid have 0 bytes. */
+size_t tilemix_cache4_block_bytes(int d);
+size_t tilemix_cache4_bytes(int64_t pages, int page_size, int kv_heads, int d);
+
+/* Rotates queries and keys by their positions and writes keys and values to the
+ * cache, in one pass. The first rotary_dim features (even, 0 .. d) of a head are
+ * turned by the angles of its token's row of cos_sin ([positions][rotary_dim]
+ * floats: rotary_dim / 2 cosines, then as many sines; rotary_dim 0: not read):
+ * (y1, y2) = (x1 cos - x2 sin, x2 cos + x1 sin), fp32, each product rounded, of
+ * the features i and i + rotary_dim / 2, or with `interleaved` 2 i and 2 i + 1.
+ * Q (optional with Q_out; Q_out may be Q) -> Q_out, K -> K_out (optional; may be K)
+ * rounded to dtype; the cache takes the keys before that rounding. V is cached as
+ * it is. Token t goes to slots[t]; a slot outside the cache (a negative one, say,
+ * for a padded row) caches nothing. A token whose position is outside the table is
+ * passed over: neither cached nor rotated. Two tokens of one call must not have
+ * the same slot: which bytes of which of them stay is not defined. tokens 0:
+ * nothing to do. */
+typedef struct TileMixCache4AppendArgs {
+    const uint16_t* Q;
+    const uint16_t* K;
+    const uint16_t* V;
+    uint16_t* Q_out;
+    uint16_t* K_out;
+    const float* cos_sin;
+    const int32_t* token_positions; /* [tokens] */
+    const int64_t* slots;           /* [tokens] */
+    uint8_t* cache;
+    int64_t pages;
+    int page_size;
+    int tokens;
+    int q_heads; /* not read without Q */
+    int kv_heads;
+    int d;
+    int dtype;
+    int rotary_dim;
+    int interleaved;
+    int positions; /* rows of cos_sin */
+    int64_t q_row_stride;
+    int64_t k_row_stride;
+    int64_t v_row_stride;
+    int64_t q_out_row_stride;
+    int64_t k_out_row_stride;
+    int64_t q_head_stride;
+    int64_t k_head_stride;
+    int64_t v_head_stride;
+    int64_t q_out_head_stride;
+    int64_t k_out_head_stride;
+} TileMixCache4AppendArgs;
+
+int tilemix_cache4_append(const TileMixCache4AppendArgs* args, void* stream);
+
+/* Cached rows back in 16 bits, e.g. the context of a prompt's next chunk for
+ * tilemix_attention_packed: K_out / V_out [tokens][kv_heads][d] (either may be
+ * NULL) receive the values at slots[t], rounded to dtype; a row whose slot is
+ * outside the cache is left as it was. tokens 0: nothing to do. */
+typedef struct TileMixCache4GatherArgs {
+    const uint8_t* cache;
+    const int64_t* slots; /* [tokens] */
+    uint16_t* K_out;
+    uint16_t* V_out;
+    int64_t pages;
+    int page_size;
+    int tokens;
+    int kv_heads;
+    int d;
+    int dtype;
+    int64_t k_row_stride;
+    int64_t v_row_stride;
+    int64_t k_head_stride;
+    int64_t v_head_stride;
+} TileMixCache4GatherArgs;
+
+int tilemix_cache4_gather(const TileMixCache4GatherArgs* args, void* stream);
+
+/* One decode step over the cache: O[b] = softmax(score_scale * q[b] K_b^T) V_b
+ * for the query token of each of `batch` sequences ([batch][q_heads][d]), whose
+ * lengths[b] cached tokens lie in the pages block_table[b * table_stride + i], i =
+ * 0 .. ceil(lengths[b] / page_size) - 1 (table_stride 0: max_pages). A sequence of
+ * length <= 0 becomes 0; lengths past max_pages * page_size end there; the tokens
+ * of a page number outside the cache are left out. What a cache holds past a
+ * sequence's length is not used.
+ * `workspace`: tilemix_attention_cache4_workspace_bytes() bytes of device memory,
+ * 16-byte aligned, set to zero once before its first call; it can serve calls of
+ * any shape, one after the other (on one stream, or ordered by events; captured
+ * calls that share one must not be replayed at once). Results do not depend on
+ * what other calls left in it. Sums are taken in an order that lengths and
+ * sizes decide: the same call gives the same bits. */
+typedef struct TileMixCache4AttentionArgs {
+    const uint16_t* Q;
+    uint16_t* O;
+    const uint8_t* cache;
+    const int32_t* block_table;
+    const int32_t* lengths; /* [batch] */
+    void* workspace;
+    size_t workspace_bytes;
+    int64_t pages;
+    int64_t table_stride;
+    int page_size;
+    int max_pages;
+    int batch;
+    int q_heads;
+    int kv_heads;
+    int d;
+    int dtype;
+    float score_scale;
+    int64_t q_row_stride;
+    int64_t o_row_stride;
+    int64_t q_head_stride;
+    int64_t o_head_stride;
+} TileMixCache4AttentionArgs;
+
+size_t tilemix_attention_cache4_workspace_bytes(void);
+int tilemix_attention_cache4(const TileMixCache4AttentionArgs* args, void* stream);
+
 /* FFI mirrors of the constexpr sizing helpers of attention_fused.h:21-45, for
  * callers that cannot evaluate C++ constexpr functions. */
 size_t tilemix_routing_words_per_row_c(int N, int key_tiles_per_group);

@@ -47,7 +47,7 @@ DEVICE_FLAGS = [
 # (source, object, extra flags): the attention kernels are compiled once per
 # head-dimension class, in parallel.
 LIB_UNITS = [("attention.hip", f"attention_dc{dc}.o", [f"-DTILEMIX_DC={dc}"]) for dc in (4, 3, 2, 1)] + [
-    (name, name + ".o", []) for name in ("decode.hip", "attention.hip", "quantize.hip", "routing.hip")]
+    (name, name + ".o", []) for name in ("packed_attention.hip", "decode.hip", "attention.hip", "cache4_attention.hip", "cache4.hip", "quantize.hip", "routing.hip")]
 
 
 def _run(cmd: list[str]) -> None:

@@ -1,0 +1,444 @@
+// Writing and reading the paged 4-bit key/value cache (tilemix_cache4_append,
+// tilemix_cache4_gather) for gfx950. Both are bound by memory: every input is
+// read once and every output written once; the formulas are in
+// include/tilemix_capi.h and the layout of a block in serving.h.
+//
+// A team of lanes - 8 for d <= 64, 16 above - holds one token's row of one head,
+// 8 features a lane (16 bytes), so that a rotation's partner features are one more
+// 16-byte load that hits the cache (where half the rotated features are a multiple
+// of 8; else single values) and a group's extremes are three DPP steps. The teams of
+// a wave hold consecutive tokens of the same head: their key codes are one run of
+// the block, and their 16-bit pieces of a value row lie side by side, so that a
+// store touches 8 bytes of each line instead of 2. The waves of a workgroup take
+// different heads of the same tokens, with the cosines and sines kept in registers.
+
+#include "serving.h"
+#include "tilemix_capi.h"
+
+#include <algorithm>
+#include <type_traits>
+
+namespace tilemix {
+namespace {
+
+constexpr int kCacheThreads = 256;
+constexpr int kCacheWaves = kCacheThreads / kWave;
+
+struct TokenRows {
+    const std::uint16_t* in;
+    std::uint16_t* out;
+    Rows in_rows, out_rows;
+};
+
+struct AppendParams {
+    TokenRows q, k, v;
+    const float* cos_sin;
+    const std::int32_t* token_positions;
+    const std::int64_t* slots;
+    Cache cache;
+    int tokens, positions;
+    int q_heads, kv_heads;
+    int d, rotary, half;
+    int interleaved;
+    int vector_partner;  // half is a multiple of 8
+    int heads_per_wave;
+};
+
+struct GatherParams {
+    TokenRows k, v;
+    const std::int64_t* slots;
+    Cache cache;
+    int tokens;
+    int kv_heads;
+    int d;
+    int heads_per_wave;
+};
+
+// Minimum / maximum / sum over the 8 lanes of a group (DPP steps inside rows of 16 lanes).
+template <typename F>
+__device__ __forceinline__ float over_8_lanes(float x, F&& f) {
+    auto step = [&](auto control) {
+        constexpr int kControl = decltype(control)::value;
+        return __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, x), kControl, 0xf, 0xf, false));
+    };
+    x = f(x, step(std::integral_constant<int, 0xb1>{}));   // lane ^ 1
+    x = f(x, step(std::integral_constant<int, 0x4e>{}));   // lane ^ 2
+    return f(x, step(std::integral_constant<int, 0x141>{}));  // mirrored within 8
+}
+
+// Where the cache has a slot: byte offset of head 0's block and the token's number in it.
+struct Place {
+    std::int64_t block;
+    int t;
+    bool ok;
+};
+__device__ __forceinline__ Place place_of(const Cache& cache, std::int64_t slot) {
+    Place at;
+    at.ok = slot >= 0 && slot < cache.pages * cache.page_size;
+    const std::int64_t page = at.ok ? slot / cache.page_size : 0;
+    const int inside = at.ok ? static_cast<int>(slot - page * cache.page_size) : 0;
+    at.block = page * cache.page_bytes + static_cast<std::int64_t>(inside / kCacheKeys) * cache_block_bytes(cache.groups);
+    at.t = inside % kCacheKeys;
+    return at;
+}
+
+// Product rounded to fp32 before anything is added to it: the compiler would
+// contract it into an fma, and the rotated values, hence the codes, would depend on which.
+__device__ __forceinline__ float rounded_product(float a, float b) {
+    float product = a * b;
+    asm("" : "+v"(product));
+    return product;
+}
+
+template <bool kBf16>
+__device__ __forceinline__ void unpack8(uint4v raw, float (&x)[8]) {
+#pragma unroll
+    for (int w = 0; w < 4; ++w) {
+        x[2 * w] = half_of<kBf16, 0>(raw[w]);
+        x[2 * w + 1] = half_of<kBf16, 1>(raw[w]);
+    }
+}
+template <bool kBf16>
+__device__ __forceinline__ uint4v pack8(const float (&x)[8]) {
+    return uint4v{pack_pair<kBf16>(x[0], x[1]), pack_pair<kBf16>(x[2], x[3]), pack_pair<kBf16>(x[4], x[5]),
+                  pack_pair<kBf16>(x[6], x[7])};
+}
+
+template <int kGroups, bool kBf16>
+__global__ __launch_bounds__(kCacheThreads) void cache4_append_kernel(const AppendParams p) {
+    constexpr int kTeam = 8 * kGroups;
+    constexpr int kTokens = kWave / kTeam;  // of a workgroup
+    const int lane = threadIdx.x & (kWave - 1);
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int token = blockIdx.x * kTokens + lane / kTeam;
+    const int chunk = lane % kTeam;  // of 8 features
+    const int f0 = 8 * chunk;
+    const int d = p.d;
+
+    bool valid = token < p.tokens;  // and its position is in the table
+    Place at{0, 0, false};
+    float cosine[8], sine[8];  // per feature: y = x cosine + partner sine, the sign in the sine
+    const bool turned = f0 < p.rotary;
+    int partner = f0;  // first feature of the partners (vector_partner)
+    if (turned && !p.interleaved) partner = f0 < p.half ? f0 + p.half : f0 - p.half;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) cosine[e] = 1.0f, sine[e] = 0.0f;
+    if (valid) {
+        at = place_of(p.cache, p.slots[token]);
+        if (p.rotary > 0) {
+            const int position = p.token_positions[token];
+            valid = position >= 0 && position < p.positions;
+            const float* const row = p.cos_sin + static_cast<std::int64_t>(valid ? position : 0) * p.rotary;
+            if (valid) {
+#pragma unroll
+                for (int e = 0; e < 8; ++e) {
+                    const int f = f0 + e;
+                    if (f < p.rotary) {
+                        const bool second = p.interleaved ? f & 1 : f >= p.half;
+                        const int angle = p.interleaved ? f >> 1 : second ? f - p.half : f;
+                        cosine[e] = row[angle];
+                        sine[e] = second ? row[p.half + angle] : -row[p.half + angle];
+                    }
+                }
+            }
+        }
+    }
+    const bool live = valid && f0 < d;     // holds values
+    const bool cached = valid && at.ok;    // writes to the cache, code 0 past d
+    const int place = cache_place(at.t);
+
+    const int first = (blockIdx.y * kCacheWaves + wave) * p.heads_per_wave;
+    const int last = min(first + p.heads_per_wave, p.q_heads + 2 * p.kv_heads);
+    // Rows of queries, then keys, then values.
+    enum Kind { kQuery, kKey, kValue };
+    struct Head {
+        TokenRows rows;
+        int index;
+        Kind kind;
+    };
+    auto head_at = [&](int n) __attribute__((always_inline)) {
+        if (n < p.q_heads) return Head{p.q, n, kQuery};
+        if (n < p.q_heads + p.kv_heads) return Head{p.k, n - p.q_heads, kKey};
+        return Head{p.v, n - p.q_heads - p.kv_heads, kValue};
+    };
+    struct Row {
+        uint4v own, other;
+    };
+    auto load = [&](int n) __attribute__((always_inline)) {
+        Row row{};
+        const Head head = head_at(n);
+        if (live) {
+            const std::uint16_t* const x = head.rows.in + token * head.rows.in_rows.row + head.index * head.rows.in_rows.head;
+            row.own = *reinterpret_cast<const uint4v*>(x + f0);
+            if (head.kind != kValue && turned && p.vector_partner) row.other = *reinterpret_cast<const uint4v*>(x + partner);
+        }
+        return row;
+    };
+    auto take = [&](int n, const Row& row) __attribute__((always_inline)) {
+        const Head head = head_at(n);
+        float x[8];
+        unpack8<kBf16>(row.own, x);
+        if (head.kind != kValue && p.rotary > 0) {
+            float other[8];
+            if (p.interleaved) {
+#pragma unroll
+                for (int e = 0; e < 8; ++e) other[e] = x[e ^ 1];
+            } else if (p.vector_partner) {
+                unpack8<kBf16>(row.other, other);
+            } else {
+                const std::uint16_t* const in = head.rows.in + token * head.rows.in_rows.row + head.index * head.rows.in_rows.head;
+#pragma unroll
+                for (int e = 0; e < 8; ++e) {
+                    const int f = f0 + e;
+                    other[e] = live && f < p.rotary ? half_of<kBf16, 0>(in[f < p.half ? f + p.half : f - p.half]) : 0.0f;
+                }
+            }
+#pragma unroll
+            for (int e = 0; e < 8; ++e)
+                if (f0 + e < p.rotary) x[e] = rounded_product(x[e], cosine[e]) + rounded_product(other[e], sine[e]);
+        }
+        if (head.rows.out && live) {
+            std::uint16_t* const y = head.rows.out + token * head.rows.out_rows.row + head.index * head.rows.out_rows.head;
+            *reinterpret_cast<uint4v*>(y + f0) = pack8<kBf16>(x);
+        }
+        if (head.kind == kQuery) return;
+        // Extremes of the group; `zero` becomes NaN with any value that is not finite.
+        float low = INFINITY, high = -INFINITY, zero = 0.0f;
+        if (live) {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                low = fminf(low, x[e]);
+                high = fmaxf(high, x[e]);
+                zero = __builtin_fmaf(x[e], 0.0f, zero);
+            }
+        }
+        low = over_8_lanes(low, [](float a, float b) { return fminf(a, b); });
+        high = over_8_lanes(high, [](float a, float b) { return fmaxf(a, b); });
+        zero = over_8_lanes(zero, [](float a, float b) { return a + b; });
+        const float minimum = half_of<true, 1>(pack_pair<true>(0.0f, low));
+        std::uint32_t params = pack_pair<true>((high - minimum) / 15.0f, minimum);
+        const float scale = half_of<true, 0>(params);
+        const bool finite = zero == 0.0f && scale < INFINITY;
+        const bool coded = finite && scale >= kLeastScale;
+        if (!finite) params = 0x7fc07fc0u;
+        else if (!coded) params &= 0xffff0000u;
+        const float recip = 1.0f / scale;
+        std::uint32_t code[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            const float steps = __builtin_rintf(quotient(x[e] - minimum, scale, recip));
+            code[e] = coded && live ? static_cast<std::uint32_t>(fminf(fmaxf(steps, 0.0f), 15.0f)) : 0u;
+        }
+        if (!cached) return;
+        std::uint8_t* const block = p.cache.data + at.block + head.index * p.cache.head_bytes;
+        if (head.kind == kKey) {
+            std::uint32_t word = 0;
+#pragma unroll
+            for (int e = 0; e < 8; ++e) word |= code[e] << (4 * (e / 2) + 16 * (e % 2));
+            const int m = chunk >> 3, g = (chunk >> 1) & 3, w = chunk & 1;
+            reinterpret_cast<std::uint32_t*>(block)[8 * kGroups * at.t + 2 * kGroups * g + 2 * m + w] = word;
+        } else {
+            auto* const quarters = reinterpret_cast<std::uint16_t*>(block + cache_values_at(kGroups)) + place;
+#pragma unroll
+            for (int half = 0; half < 2; ++half)
+                quarters[(2 * chunk + half) * kCacheKeys] =
+                    static_cast<std::uint16_t>(code[4 * half] | (code[4 * half + 1] << 4) | (code[4 * half + 2] << 8) |
+                                               (code[4 * half + 3] << 12));
+        }
+        if ((chunk & 7) == 0)
+            reinterpret_cast<std::uint32_t*>(block + (head.kind == kKey ? cache_key_params_at(kGroups) : cache_value_params_at(kGroups)))
+                [(chunk >> 3) * kCacheKeys + place] = params;
+    };
+    constexpr int kBatch = 4;
+    for (int n = first; n < last; n += kBatch) {
+        Row rows[kBatch];
+#pragma unroll
+        for (int b = 0; b < kBatch; ++b)
+            if (n + b < last) rows[b] = load(n + b);
+#pragma unroll
+        for (int b = 0; b < kBatch; ++b)
+            if (n + b < last) take(n + b, rows[b]);
+    }
+}
+
+template <int kGroups, bool kBf16>
+__global__ __launch_bounds__(kCacheThreads) void cache4_gather_kernel(const GatherParams p) {
+    constexpr int kTeam = 8 * kGroups;
+    constexpr int kTokens = kWave / kTeam;
+    const int lane = threadIdx.x & (kWave - 1);
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int token = blockIdx.x * kTokens + lane / kTeam;
+    const int chunk = lane % kTeam, f0 = 8 * chunk;
+    if (token >= p.tokens || f0 >= p.d) return;
+    const Place at = place_of(p.cache, p.slots[token]);
+    if (!at.ok) return;
+    const int place = cache_place(at.t);
+    const int m = chunk >> 3, g = (chunk >> 1) & 3, w = chunk & 1;
+    const int heads_k = p.k.out ? p.kv_heads : 0, heads = heads_k + (p.v.out ? p.kv_heads : 0);
+    const int first = (blockIdx.y * kCacheWaves + wave) * p.heads_per_wave;
+    const int last = min(first + p.heads_per_wave, heads);
+    struct Codes {
+        std::uint32_t params, low, high;  // a key's word is in low
+    };
+    auto load = [&](int n) __attribute__((always_inline)) {
+        const bool key = n < heads_k;
+        const std::uint8_t* const block = p.cache.data + at.block + (key ? n : n - heads_k) * p.cache.head_bytes;
+        Codes c{};
+        if (key) {
+            c.low = reinterpret_cast<const std::uint32_t*>(block)[8 * kGroups * at.t + 2 * kGroups * g + 2 * m + w];
+        } else {
+            const auto* const quarters = reinterpret_cast<const std::uint16_t*>(block + cache_values_at(kGroups)) + place;
+            c.low = quarters[2 * chunk * kCacheKeys];
+            c.high = quarters[(2 * chunk + 1) * kCacheKeys];
+        }
+        c.params = reinterpret_cast<const std::uint32_t*>(
+            block + (key ? cache_key_params_at(kGroups) : cache_value_params_at(kGroups)))[m * kCacheKeys + place];
+        return c;
+    };
+    auto take = [&](int n, const Codes& c) __attribute__((always_inline)) {
+        const bool key = n < heads_k;
+        const TokenRows rows = key ? p.k : p.v;
+        const float scale = half_of<true, 0>(c.params), minimum = half_of<true, 1>(c.params);
+        float x[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            const std::uint32_t code = key ? c.low >> (4 * (e / 2) + 16 * (e % 2)) : (e < 4 ? c.low : c.high) >> (4 * (e % 4));
+            x[e] = __builtin_fmaf(scale, static_cast<float>(code & 15u), minimum);
+        }
+        std::uint16_t* const y = rows.out + token * rows.out_rows.row + (key ? n : n - heads_k) * rows.out_rows.head;
+        *reinterpret_cast<uint4v*>(y + f0) = pack8<kBf16>(x);
+    };
+    constexpr int kBatch = 4;
+    for (int n = first; n < last; n += kBatch) {
+        Codes codes[kBatch];
+#pragma unroll
+        for (int b = 0; b < kBatch; ++b)
+            if (n + b < last) codes[b] = load(n + b);
+#pragma unroll
+        for (int b = 0; b < kBatch; ++b)
+            if (n + b < last) take(n + b, codes[b]);
+    }
+}
+
+// Heads that one wave takes in turn: enough waves to fill the device first.
+int heads_per_wave(std::int64_t token_groups, int heads) {
+    constexpr int kWavesWanted = 4096, kMost = 16;
+    return static_cast<int>(std::clamp<std::int64_t>(token_groups * heads / kWavesWanted, 1, std::min(heads, kMost)));
+}
+
+template <int kGroups>
+hipError_t launch_append(AppendParams p, bool bf16, hipStream_t stream) {
+    constexpr int kTokens = kWave / (8 * kGroups);
+    const unsigned token_groups = static_cast<unsigned>((p.tokens - 1) / kTokens + 1);
+    const int heads = p.q_heads + 2 * p.kv_heads;
+    p.heads_per_wave = heads_per_wave(token_groups, heads);
+    const int per_group = kCacheWaves * p.heads_per_wave;
+    const dim3 grid(token_groups, static_cast<unsigned>((heads + per_group - 1) / per_group));
+    if (grid.y > 65535) return hipErrorInvalidConfiguration;
+    if (bf16)
+        cache4_append_kernel<kGroups, true><<<grid, kCacheThreads, 0, stream>>>(p);
+    else
+        cache4_append_kernel<kGroups, false><<<grid, kCacheThreads, 0, stream>>>(p);
+    return hipGetLastError();
+}
+
+template <int kGroups>
+hipError_t launch_gather(GatherParams p, bool bf16, hipStream_t stream) {
+    constexpr int kTokens = kWave / (8 * kGroups);
+    const unsigned token_groups = static_cast<unsigned>((p.tokens - 1) / kTokens + 1);
+    const int heads = (p.k.out ? p.kv_heads : 0) + (p.v.out ? p.kv_heads : 0);
+    p.heads_per_wave = heads_per_wave(token_groups, heads);
+    const int per_group = kCacheWaves * p.heads_per_wave;
+    const dim3 grid(token_groups, static_cast<unsigned>((heads + per_group - 1) / per_group));
+    if (grid.y > 65535) return hipErrorInvalidConfiguration;
+    if (bf16)
+        cache4_gather_kernel<kGroups, true><<<grid, kCacheThreads, 0, stream>>>(p);
+    else
+        cache4_gather_kernel<kGroups, false><<<grid, kCacheThreads, 0, stream>>>(p);
+    return hipGetLastError();
+}
+
+bool dtype_ok(int dtype) { return dtype == TILEMIX_DTYPE_F16 || dtype == TILEMIX_DTYPE_BF16; }
+
+}  // namespace
+}  // namespace tilemix
+
+extern "C" std::size_t tilemix_cache4_block_bytes(int d) {
+    if (d <= 0 || d > tilemix::kMaxHeadDim || d % 8 != 0) return 0;
+    return static_cast<std::size_t>(tilemix::cache_block_bytes(tilemix::cache_groups(d)));
+}
+
+extern "C" std::size_t tilemix_cache4_bytes(std::int64_t pages, int page_size, int kv_heads, int d) {
+    alignas(16) static const std::uint8_t any[16] = {};  // an address that passes the check
+    tilemix::Cache cache;
+    if (tilemix::make_cache(cache, any, pages, page_size, kv_heads, d) != hipSuccess) return 0;
+    return static_cast<std::size_t>(cache.pages) * static_cast<std::size_t>(cache.page_bytes);
+}
+
+extern "C" int tilemix_cache4_append(const TileMixCache4AppendArgs* args, void* stream) {
+    using namespace tilemix;
+    if (!args) return hipErrorInvalidValue;
+    const TileMixCache4AppendArgs& a = *args;
+    AppendParams p{};
+    const hipError_t cache_ok = make_cache(p.cache, a.cache, a.pages, a.page_size, a.kv_heads, a.d);
+    if (cache_ok != hipSuccess) return cache_ok;
+    if (a.tokens < 0 || !dtype_ok(a.dtype) || a.rotary_dim < 0 || a.rotary_dim > a.d || a.rotary_dim % 2 != 0 ||
+        (a.Q && a.q_heads <= 0) || (!a.Q) != (!a.Q_out) ||
+        (a.rotary_dim > 0 && (a.positions <= 0 || !a.cos_sin || !a.token_positions)))
+        return hipErrorInvalidValue;
+    p.q_heads = a.Q ? a.q_heads : 0;
+    if (p.q_heads > 0x3fffffff || a.kv_heads > 0x1fffffff) return hipErrorInvalidValue;
+    p.q.in = a.Q, p.q.out = a.Q_out;
+    p.k.in = a.K, p.k.out = a.K_out;
+    p.v.in = a.V, p.v.out = nullptr;
+    if ((a.Q && (!make_rows(p.q.in_rows, a.Q, a.tokens, a.q_heads, a.d, a.q_row_stride, a.q_head_stride, 8) ||
+                 !make_rows(p.q.out_rows, a.Q_out, a.tokens, a.q_heads, a.d, a.q_out_row_stride, a.q_out_head_stride, 8))) ||
+        !make_rows(p.k.in_rows, a.K, a.tokens, a.kv_heads, a.d, a.k_row_stride, a.k_head_stride, 8) ||
+        (a.K_out && !make_rows(p.k.out_rows, a.K_out, a.tokens, a.kv_heads, a.d, a.k_out_row_stride, a.k_out_head_stride, 8)) ||
+        !make_rows(p.v.in_rows, a.V, a.tokens, a.kv_heads, a.d, a.v_row_stride, a.v_head_stride, 8))
+        return hipErrorInvalidValue;
+    if (a.tokens == 0) return hipSuccess;
+    if (!a.slots) return hipErrorInvalidValue;
+    p.cos_sin = a.cos_sin;
+    p.token_positions = a.token_positions;
+    p.slots = a.slots;
+    p.tokens = a.tokens;
+    p.positions = a.positions;
+    p.kv_heads = a.kv_heads;
+    p.d = a.d;
+    p.rotary = a.rotary_dim;
+    p.half = a.rotary_dim / 2;
+    p.interleaved = a.interleaved != 0;
+    p.vector_partner = !p.interleaved && p.half % 8 == 0;
+    const hipError_t found = check_device();
+    if (found != hipSuccess) return found;
+    const bool bf16 = a.dtype == TILEMIX_DTYPE_BF16;
+    return p.cache.groups == 1 ? launch_append<1>(p, bf16, static_cast<hipStream_t>(stream))
+                               : launch_append<2>(p, bf16, static_cast<hipStream_t>(stream));
+}
+
+extern "C" int tilemix_cache4_gather(const TileMixCache4GatherArgs* args, void* stream) {
+    using namespace tilemix;
+    if (!args) return hipErrorInvalidValue;
+    const TileMixCache4GatherArgs& a = *args;
+    GatherParams p{};
+    const hipError_t cache_ok = make_cache(p.cache, a.cache, a.pages, a.page_size, a.kv_heads, a.d);
+    if (cache_ok != hipSuccess) return cache_ok;
+    if (a.tokens < 0 || !dtype_ok(a.dtype) || a.kv_heads > 0x1fffffff) return hipErrorInvalidValue;
+    if (a.tokens == 0) return hipSuccess;
+    if (!a.slots || (!a.K_out && !a.V_out)) return hipErrorInvalidValue;
+    p.k.out = a.K_out;
+    p.v.out = a.V_out;
+    if ((a.K_out && !make_rows(p.k.out_rows, a.K_out, a.tokens, a.kv_heads, a.d, a.k_row_stride, a.k_head_stride, 8)) ||
+        (a.V_out && !make_rows(p.v.out_rows, a.V_out, a.tokens, a.kv_heads, a.d, a.v_row_stride, a.v_head_stride, 8)))
+        return hipErrorInvalidValue;
+    p.slots = a.slots;
+    p.tokens = a.tokens;
+    p.kv_heads = a.kv_heads;
+    p.d = a.d;
+    const hipError_t found = check_device();
+    if (found != hipSuccess) return found;
+    const bool bf16 = a.dtype == TILEMIX_DTYPE_BF16;
+    return p.cache.groups == 1 ? launch_gather<1>(p, bf16, static_cast<hipStream_t>(stream))
+                               : launch_gather<2>(p, bf16, static_cast<hipStream_t>(stream));
+}

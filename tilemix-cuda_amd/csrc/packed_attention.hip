@@ -1,0 +1,570 @@
+// Attention of packed sequences with grouped query heads for gfx950
+// (tilemix_attention_packed): fp16 / bf16, causal with rows aligned at the end
+// of their sequence's keys, or not causal.
+//
+// O[t, h] = sum_j p_j v[j, h / G],  p = softmax_j(scale q[t, h] . k[j, h / G]).
+//
+//  * A workgroup of four waves owns 32 query rows per wave: kTeam heads of one
+//    key head (kTeam = the largest power of two up to 4 that divides G) x
+//    128 / kTeam tokens. Waves of different heads with the same tokens share each
+//    K / V tile and end at the same diagonal, so a causal walk has less masked
+//    work than with 128 tokens of one head, and a short sequence fills its
+//    workgroup.
+//  * Which tokens a workgroup takes is found on the device (find_block), from the
+//    lengths, blocks of more key tiles first: the host knows neither the lengths
+//    nor the longest.
+//  * Scores, softmax and P.V as in attention_kernel (attention.hip): S^T = K Q^T
+//    and O^T = V^T P^T on 32x32x16 MFMAs, probabilities kept in registers, K / V
+//    tiles by LDS DMA.
+//  * Every tile is addressed through a buffer that starts at its first row and ends
+//    after the sequence's last, so rows of the next sequence read as zero and a
+//    sequence may pass 2 GiB.
+
+#include "attention_tiles.h"
+#include "serving.h"
+#include "tilemix_capi.h"
+
+#include <algorithm>
+#include <cmath>
+
+namespace tilemix {
+namespace {
+
+constexpr int kBlockRows = 128;  // query rows (tokens x heads) of a workgroup
+
+struct PackedParams {
+    const std::uint16_t* Q;
+    const std::uint16_t* K;
+    const std::uint16_t* V;
+    std::uint16_t* O;
+    const std::int32_t* q_starts;
+    const std::int32_t* k_starts;
+    std::int64_t q_row, k_row, v_row, o_row;      // elements between tokens
+    std::int64_t q_head, k_head, v_head, o_head;  // and between heads
+    int batch;
+    int q_tokens, k_tokens;
+    int kv_heads;
+    int group;       // query heads per key head
+    int chunks;      // group / team
+    int team_shift;  // log2 of the heads of a workgroup
+    int d;
+    int causal;
+    int negate;  // score_scale < 0: Q is negated
+    float score_log2;  // |score_scale| log2(e)
+};
+
+// ------------------------------------------------------------ work items
+
+struct Sequence {
+    int q0, q_len, k0, k_len;
+};
+
+// Bounds of sequence b, inside the tensors whatever the starts hold.
+__device__ __forceinline__ Sequence sequence_at(const PackedParams& p, int b) {
+    Sequence s;
+    s.q0 = min(max(p.q_starts[b], 0), p.q_tokens);
+    s.q_len = min(max(p.q_starts[b + 1], s.q0), p.q_tokens) - s.q0;
+    s.k0 = min(max(p.k_starts[b], 0), p.k_tokens);
+    s.k_len = min(max(p.k_starts[b + 1], s.k0), p.k_tokens) - s.k0;
+    return s;
+}
+
+// Sum over the wave's lanes, in every lane (DPP steps as in wave_max_bits).
+__device__ __forceinline__ int wave_sum(int v) {
+    v += __builtin_amdgcn_update_dpp(0, v, 0xb1, 0xf, 0xf, false);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x4e, 0xf, 0xf, false);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x141, 0xf, 0xf, false);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x140, 0xf, 0xf, false);
+    int a = v, b = v;
+    asm volatile("s_nop 1\n\tv_permlane16_swap_b32 %0, %1" : "+v"(a), "+v"(b));
+    v = a + b;
+    a = v;
+    b = v;
+    asm volatile("s_nop 1\n\tv_permlane32_swap_b32 %0, %1" : "+v"(a), "+v"(b));
+    return __builtin_amdgcn_readfirstlane(a + b);
+}
+
+// Blocks of `tokens` query tokens of a sequence that walk at least `tiles` key tiles.
+__device__ __forceinline__ int blocks_walking(const Sequence& s, int tokens, int tiles, bool causal) {
+    const int blocks = (s.q_len + tokens - 1) / tokens;
+    if (tiles <= 0) return blocks;
+    const std::int64_t keys = std::int64_t{kTileKeys} * (tiles - 1) + 1;  // the fewest of so many tiles
+    if (s.k_len < keys) return 0;
+    if (!causal) return blocks;
+    // Block j sees keys up to k_len - q_len + (j + 1) tokens.
+    const std::int64_t first = (keys - (s.k_len - s.q_len) + tokens - 1) / tokens - 1;
+    return first <= 0 ? blocks : static_cast<int>(first < blocks ? blocks - first : 0);
+}
+
+// The sequence and block of work item `slot`, items of more key tiles first
+// (the last to start are the shortest; a long walk that starts last would run
+// alone); false past the last. Wave-uniform.
+__device__ __forceinline__ bool find_block(const PackedParams& p, int slot, int tokens, int lane, Sequence& found, int& block) {
+    const bool causal = p.causal != 0;
+    if (p.batch == 1) {
+        found = sequence_at(p, 0);
+        const int blocks = (found.q_len + tokens - 1) / tokens;
+        block = blocks - 1 - slot;
+        return slot < blocks;
+    }
+    Sequence mine{0, 0, 0, 0};
+    if (lane < p.batch) mine = sequence_at(p, lane);
+    const bool few = p.batch <= kWave;
+    auto count = [&](int tiles) {
+        int n = blocks_walking(mine, tokens, tiles, causal);
+        if (!few)
+            for (int b = lane + kWave; b < p.batch; b += kWave) n += blocks_walking(sequence_at(p, b), tokens, tiles, causal);
+        return wave_sum(n);
+    };
+    if (count(0) <= slot) return false;
+    // The most tiles of which more than `slot` blocks have as many.
+    int low = 0, high = (p.k_tokens + kTileKeys - 1) / kTileKeys + 1;
+    while (high - low > 1) {
+        const int middle = (low + high) >> 1;
+        if (count(middle) > slot)
+            low = middle;
+        else
+            high = middle;
+    }
+    int rest = slot - count(low + 1);  // among the blocks of exactly `low` tiles
+    for (int base = 0;; base += kWave) {
+        const int b = base + lane;
+        Sequence s{0, 0, 0, 0};
+        if (b < p.batch) s = sequence_at(p, b);
+        const int above = blocks_walking(s, tokens, low + 1, causal);
+        const int here = blocks_walking(s, tokens, low, causal) - above;
+        int before = here;  // inclusive prefix over the lanes
+#pragma unroll
+        for (int step = 1; step < kWave; step <<= 1) {
+            const int other = __shfl_up(before, step);
+            if (lane >= step) before += other;
+        }
+        const std::uint64_t past = __ballot(before > rest);
+        if (past) {
+            const int at = __builtin_ctzll(past);
+            found.q0 = __builtin_amdgcn_readlane(s.q0, at);
+            found.q_len = __builtin_amdgcn_readlane(s.q_len, at);
+            found.k0 = __builtin_amdgcn_readlane(s.k0, at);
+            found.k_len = __builtin_amdgcn_readlane(s.k_len, at);
+            // Blocks of a sequence walk more tiles the later they are.
+            const int blocks = (found.q_len + tokens - 1) / tokens;
+            block = blocks - 1 - __builtin_amdgcn_readlane(above, at) - (rest - __builtin_amdgcn_readlane(before - here, at));
+            return true;
+        }
+        rest -= __builtin_amdgcn_readlane(before, kWave - 1);
+    }
+}
+
+// ------------------------------------------------------- 16-bit arithmetic
+
+template <bool kBf16>
+__device__ __forceinline__ float16v mfma_32x32x16(uint4v a, uint4v b, float16v c) {
+    if constexpr (kBf16)
+        return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf8v, a), __builtin_bit_cast(bf8v, b), c, 0, 0, 0);
+    else
+        return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(half8, a), __builtin_bit_cast(half8, b), c, 0, 0, 0);
+}
+
+// sum + both halves of a pair.
+template <bool kBf16>
+__device__ __forceinline__ float add_pair(std::uint32_t pair, float sum) {
+    if constexpr (kBf16)
+        return __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(bf2v, pair), bf2v{1.0f, 1.0f}, sum, false);
+    else
+        return __builtin_amdgcn_fdot2(__builtin_bit_cast(half2v, pair), half2v{1.0f16, 1.0f16}, sum, false);
+}
+
+// softmax_tile of attention.hip for either type. The row sums take exactly the
+// rounded probabilities that P.V uses: their rounding (2^-9 of each for bf16)
+// then cancels where values agree, and the rest is of the size of O's own rounding.
+template <int kOB, bool kBf16>
+__device__ __forceinline__ void softmax_rows(RowState<kOB>& st, const float16v (&x)[2], float c, uint4v (&p)[4]) {
+    const float tile = max3(block_max16(x[0]), block_max16(x[1]), block_max16(x[1])) * c;  // c >= 0
+    if (__any(tile > st.m + kLazyRescale)) {
+        float a = tile, b = tile;
+        permlane32_swap(a, b);
+        const float m_new = fmaxf(st.m, max3(a, b, b));
+        const float alpha = m_new == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(st.m - m_new);
+        st.m = m_new;
+#pragma unroll
+        for (int fb = 0; fb < kOB; ++fb) st.o[fb] *= alpha;
+        st.lsum *= alpha;
+    }
+    const float neg_m = st.m == -INFINITY ? 0.0f : -st.m;
+    float part[4];
+#pragma unroll
+    for (int ks = 0; ks < 4; ++ks) {
+        const int kb = ks >> 1, base = 8 * (ks & 1);
+#pragma unroll
+        for (int e = 0; e < 8; e += 2)
+            p[ks][e / 2] = pack_pair<kBf16>(__builtin_amdgcn_exp2f(__builtin_fmaf(x[kb][base + e], c, neg_m)),
+                                            __builtin_amdgcn_exp2f(__builtin_fmaf(x[kb][base + e + 1], c, neg_m)));
+        float sum = 0.0f;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) sum = add_pair<kBf16>(p[ks][e], sum);
+        part[ks] = sum;
+        if (ks == 1) set_priority<2>();
+    }
+    st.lsum += (part[0] + part[1]) + (part[2] + part[3]);
+}
+
+// Whether any 16-bit value of the fragment is infinite or NaN.
+template <bool kBf16>
+__device__ __forceinline__ bool not_finite(uint4v v) {
+    constexpr unsigned kExponent = kBf16 ? 0x7f80u : 0x7c00u;
+    bool any = false;
+#pragma unroll
+    for (int w = 0; w < 4; ++w)
+        any |= (v[w] & kExponent) == kExponent || (v[w] & (kExponent << 16)) == (kExponent << 16);
+    return any;
+}
+
+// What P.V takes of a value that is not finite, per half: class 0 the finite
+// values (others 0), 1 one for +inf, 2 one for -inf, 3 one for NaN.
+template <bool kBf16>
+__device__ __forceinline__ uint4v value_class(uint4v v, int which) {
+    constexpr unsigned kExponent = kBf16 ? 0x7f80u : 0x7c00u, kOne = kBf16 ? 0x3f80u : 0x3c00u;
+    uint4v out;
+#pragma unroll
+    for (int w = 0; w < 4; ++w) {
+        unsigned word = 0;
+#pragma unroll
+        for (int half = 0; half < 2; ++half) {
+            const unsigned x = (v[w] >> (16 * half)) & 0xffffu, magnitude = x & 0x7fffu;
+            const unsigned kind = magnitude < kExponent ? 0u : magnitude > kExponent ? 3u : 1u + (x >> 15);
+            const unsigned value = kind != static_cast<unsigned>(which) ? 0u : which == 0 ? x : kOne;
+            word |= value << (16 * half);
+        }
+        out[w] = word;
+    }
+    return out;
+}
+
+template <int DC, bool kBf16>
+__global__ __launch_bounds__(kThreadsPerGroup, 2) void packed_attention_kernel(const PackedParams p) {
+    using L = Layout<DC>;
+    constexpr int kDP = L::kDP;
+    constexpr int kOB = DC;
+    constexpr int kQC = kDP / 16;
+    // K | V 0 | V 1
+    __shared__ __attribute__((aligned(16))) unsigned char smem[L::kKBytes + 2 * L::kVBytes];
+    __shared__ __attribute__((aligned(16))) unsigned char lds_spare[1024];  // landing area of the spare DMA slots
+    unsigned char* const lds_k = smem;
+    unsigned char* const lds_v = smem + L::kKBytes;
+    const unsigned lds_k_address = lds_address_of(smem);
+    const unsigned lds_v_address = lds_k_address + L::kKBytes;
+    const unsigned lds_spare_address = lds_address_of(lds_spare);
+
+    const int tid = threadIdx.x;
+    const int lane = tid & (kWave - 1);
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int i = lane & 15;
+    const int q = lane & 31;
+    const int h = lane >> 5;
+    const int d = p.d;
+
+    // Consecutive workgroups go to consecutive XCDs: with eight key heads (or a
+    // multiple) each XCD keeps the K / V of its own heads in its L2.
+    const int teams = p.kv_heads * p.chunks;
+    const int team = blockIdx.x % teams, slot = blockIdx.x / teams;
+    const int kv_head = p.chunks == 1 ? team : team % p.kv_heads, chunk = p.chunks == 1 ? 0 : team / p.kv_heads;
+    const int team_heads = 1 << p.team_shift;
+    const int tokens = kBlockRows >> p.team_shift;
+    Sequence seq;
+    int block;
+    if (!find_block(p, slot, tokens, lane, seq, block)) return;
+    const int context = seq.k_len - seq.q_len;  // row i sees keys up to context + i
+    const int head = kv_head * p.group + (chunk << p.team_shift) + (wave & (team_heads - 1));
+    const int t0 = block * tokens;
+    const int tw = t0 + kRowsPerWave * (wave >> p.team_shift);  // the wave's first token
+
+    // ---------------------------------------------------------------- Q
+    uint4v qf[kQC];
+    {
+        const bool row_ok = tw + q < seq.q_len;
+        const std::uint16_t* const row = p.Q + static_cast<std::int64_t>(seq.q0 + tw + q) * p.q_row + head * p.q_head;
+#pragma unroll
+        for (int c = 0; c < kQC; ++c) {
+            const int feature = 16 * c + 8 * h;
+            qf[c] = row_ok && feature < d ? *reinterpret_cast<const uint4v*>(row + feature) : uint4v{0u, 0u, 0u, 0u};
+            if (p.negate) qf[c] ^= 0x80008000u;
+        }
+    }
+
+    // ------------------------------------------------------ tile movement
+    const int k_row_bytes = static_cast<int>(p.k_row * 2), v_row_bytes = static_cast<int>(p.v_row * 2);
+    const std::uint16_t* const Ks = p.K + static_cast<std::int64_t>(seq.k0) * p.k_row + kv_head * p.k_head;
+    const std::uint16_t* const Vs = p.V + static_cast<std::int64_t>(seq.k0) * p.v_row + kv_head * p.v_head;
+    int off_k[L::kKPerWave], off_v[L::kVPerWave];
+    unsigned dst_k[L::kKPerWave], dst_v[L::kVPerWave];
+#pragma unroll
+    for (int t = 0; t < L::kKPerWave; ++t) {
+        const int w = wave + kWavesPerGroup * t;
+        off_k[t] = w < L::kKLoads ? L::template kv_lane_offset<true>(w, lane, L::kKStride, 2 * d, k_row_bytes) : kOutOfRange;
+        dst_k[t] = w < L::kKLoads ? lds_k_address + 1024 * w : lds_spare_address;
+    }
+#pragma unroll
+    for (int t = 0; t < L::kVPerWave; ++t) {
+        const int w = wave + kWavesPerGroup * t;
+        off_v[t] = w < L::kVLoads ? L::template kv_lane_offset<false>(w, lane, L::kVStride, 2 * d, v_row_bytes) : kOutOfRange;
+        dst_v[t] = w < L::kVLoads ? lds_v_address + 1024 * w : lds_spare_address;
+    }
+    // The rows of tile j that the sequence has, as a buffer (64 rows reach under 2 GiB).
+    auto tile_rows = [&](const std::uint16_t* rows, std::int64_t row, int row_bytes, int j) {
+        const int count = min(seq.k_len - j * kTileKeys, kTileKeys);
+        return make_rsrc(rows + static_cast<std::int64_t>(j) * kTileKeys * row, (count - 1) * row_bytes + 2 * d);
+    };
+    auto issue_k = [&](int j) {
+        const int4v r = tile_rows(Ks, p.k_row, k_row_bytes, j);
+        if constexpr (L::kKLoads % kWavesPerGroup == 0) {
+            load_slots(r, dst_k[0], off_k, 0);
+        } else {
+#pragma unroll
+            for (int t = 0; t < L::kKPerWave; ++t) load_to_lds(r, dst_k[t], off_k[t], 0);
+        }
+    };
+    auto issue_v = [&](int j, int buffer) {
+        const int4v r = tile_rows(Vs, p.v_row, v_row_bytes, j);
+        const unsigned shift = buffer ? static_cast<unsigned>(L::kVBytes) : 0u;
+        if constexpr (L::kVLoads % kWavesPerGroup == 0) {
+            load_slots(r, dst_v[0] + shift, off_v, 0);
+        } else {
+#pragma unroll
+            for (int t = 0; t < L::kVPerWave; ++t)
+                load_to_lds(r, dst_v[t] == lds_spare_address ? dst_v[t] : dst_v[t] + shift, off_v[t], 0);
+        }
+    };
+    auto tile_barrier = [&]() {
+        __builtin_amdgcn_s_waitcnt(0x0f70);  // own tile loads: vmcnt(0)
+        __syncthreads();
+    };
+
+    int k_lane[kQC], v_lane[kOB];
+#pragma unroll
+    for (int c = 0; c < kQC; ++c) k_lane[c] = L::k_at(q, 32 * c + 16 * h);
+#pragma unroll
+    for (int fb = 0; fb < kOB; ++fb)
+        v_lane[fb] = L::v_at(4 * h + (i >> 2), 2 * (16 * fb + (kDP / 2) * ((lane >> 4) & 1) + 4 * (i & 3)));
+
+    // ---------------------------------------------------------- key loop
+    RowState<kOB> st;
+#pragma unroll
+    for (int fb = 0; fb < kOB; ++fb) st.o[fb] = float16v{};
+    st.lsum = 0.0f;
+    st.m = -INFINITY;
+
+    // Last key that some row of the workgroup / of the wave sees, and all rows of the wave see.
+    const int rows_end = min(t0 + tokens, seq.q_len);
+    const int group_last = p.causal ? min(context + rows_end, seq.k_len) - 1 : seq.k_len - 1;
+    const int tiles = group_last < 0 ? 0 : group_last / kTileKeys + 1;
+    const int wave_last = tw >= seq.q_len ? -1 : p.causal ? min(context + tw + kRowsPerWave, seq.k_len) - 1 : seq.k_len - 1;
+    const int all_last = p.causal ? context + tw : seq.k_len - 1;
+
+    int v_buffer = 0;
+    if (tiles > 0) {
+        issue_k(0);
+        issue_v(0, 0);
+    }
+    for (int j = 0; j < tiles; ++j) {
+        const int k0 = j * kTileKeys;
+        tile_barrier();  // K_j, V_j landed; every wave finished P.V of the previous tile
+        set_priority<2>();
+        const bool active = k0 <= wave_last;
+        const bool masked = k0 + kTileKeys - 1 > min(all_last, seq.k_len - 1);
+        float16v s[2];
+        float c = p.score_log2;
+        if (active) {
+            s[0] = float16v{};
+            s[1] = float16v{};
+            uint4v kf[3][2];
+            auto load_c = [&](int cc, uint4v (&dst)[2]) {
+#pragma unroll
+                for (int kb = 0; kb < 2; ++kb)
+                    dst[kb] = *reinterpret_cast<const uint4v*>(lds_k + 32 * L::kKStride * kb + k_lane[cc]);
+            };
+            load_c(0, kf[0]);
+            load_c(1, kf[1]);
+#pragma unroll
+            for (int cc = 0; cc < kQC; ++cc) {
+                if (cc + 2 < kQC) load_c(cc + 2, kf[(cc + 2) % 3]);
+#pragma unroll
+                for (int kb = 0; kb < 2; ++kb) s[kb] = mfma_32x32x16<kBf16>(kf[cc % 3][kb], qf[cc], s[kb]);
+                __builtin_amdgcn_sched_barrier(0);
+            }
+        }
+        // The last key that the lane's row sees, from the tile's first key of the lane.
+        int seen = (p.causal ? min(context + tw + q, seq.k_len - 1) : seq.k_len - 1) - k0 - 4 * h;
+        if (active && masked) {
+            asm volatile("" : "+v"(seen));
+#pragma unroll
+            for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+                for (int e = 0; e < 16; ++e)
+                    s[kb][e] = 32 * kb + 8 * (e >> 2) + (e & 3) > seen ? -INFINITY : s[kb][e] * c;
+            c = 1.0f;
+        }
+        tile_barrier();  // every wave finished reading K_j (and P.V of the previous tile)
+        set_priority<0>();
+        if (j + 1 < tiles) {
+            issue_k(j + 1);
+            issue_v(j + 1, v_buffer ^ 1);
+        }
+        if (active) {
+            uint4v ph[4];
+            softmax_rows<kOB, kBf16>(st, s, c, ph);
+            const unsigned char* const v_tile = lds_v + (v_buffer ? L::kVBytes : 0);
+            // V^T fragment of step t = (key step t / kOB, feature block t % kOB).
+            auto v_frag = [&](int t) {
+                const unsigned char* const lo = v_tile + 16 * L::kVStride * (t / kOB) + v_lane[t % kOB];
+                return __builtin_bit_cast(uint4v, concat(read_tr16(lo), read_tr16(lo + 8 * L::kVStride)));
+            };
+            constexpr int kSteps = 4 * kOB;
+            bool special = false;
+            if (p.causal && masked) {
+                // A row's probability of a key that it does not see is 0, but 0 times an
+                // infinite or NaN value is NaN.
+#pragma unroll
+                for (int t = 0; t < kSteps; ++t) special |= not_finite<kBf16>(v_frag(t));
+                special = __any(special);
+            }
+            if (!special) {
+                constexpr int kAhead = 3;
+                set_priority<0>();
+                uint4v vf[kAhead + 1];
+#pragma unroll
+                for (int t = 0; t < kAhead; ++t)
+                    if (t < kSteps) vf[t] = v_frag(t);
+#pragma unroll
+                for (int t = 0; t < kSteps; ++t) {
+                    if (t + kAhead < kSteps) vf[(t + kAhead) % (kAhead + 1)] = v_frag(t + kAhead);
+                    st.o[t % kOB] = mfma_32x32x16<kBf16>(vf[t % (kAhead + 1)], ph[t / kOB], st.o[t % kOB]);
+                    __builtin_amdgcn_sched_barrier(0);
+                }
+            } else {
+                // The finite values; then which of +inf, -inf and NaN the row sees, by how many.
+                constexpr std::uint32_t kOne = kBf16 ? 0x3f80u : 0x3c00u;
+                auto sees = [&](int ks) {
+                    uint4v out;
+#pragma unroll
+                    for (int e = 0; e < 8; e += 2) {
+                        const int key = 32 * (ks >> 1) + 8 * ((8 * (ks & 1) + e) >> 2) + (e & 3);
+                        out[e / 2] = (key <= seen ? kOne : 0u) | (key + 1 <= seen ? kOne << 16 : 0u);
+                    }
+                    return out;
+                };
+#pragma unroll
+                for (int fb = 0; fb < kOB; ++fb)
+#pragma unroll
+                    for (int ks = 0; ks < 4; ++ks)
+                        st.o[fb] = mfma_32x32x16<kBf16>(value_class<kBf16>(v_frag(ks * kOB + fb), 0), ph[ks], st.o[fb]);
+#pragma unroll 1
+                for (int kind = 1; kind < 4; ++kind) {
+                    const float value = kind == 1 ? INFINITY : kind == 2 ? -INFINITY : NAN;
+#pragma unroll
+                    for (int fb = 0; fb < kOB; ++fb) {
+                        float16v count{};
+#pragma unroll
+                        for (int ks = 0; ks < 4; ++ks)
+                            count = mfma_32x32x16<kBf16>(value_class<kBf16>(v_frag(ks * kOB + fb), kind), sees(ks), count);
+#pragma unroll
+                        for (int e = 0; e < 16; ++e) st.o[fb][e] += count[e] > 0.0f ? value : 0.0f;
+                    }
+                }
+            }
+        }
+        v_buffer ^= 1;
+    }
+
+    // ---------------------------------------------------------- epilogue
+    float a = st.lsum, b = st.lsum;
+    permlane32_swap(a, b);
+    const float l = a + b;
+    // 0: no key; NaN scores leave l NaN, and the row becomes NaN.
+    const float inverse = l == 0.0f ? 0.0f : 1.0f / l;
+    if (tw + q < seq.q_len) {
+        std::uint16_t* const row = p.O + static_cast<std::int64_t>(seq.q0 + tw + q) * p.o_row + head * p.o_head;
+#pragma unroll
+        for (int fb = 0; fb < kOB; ++fb)
+#pragma unroll
+            for (int r4 = 0; r4 < 4; ++r4) {
+                const int feature = (r4 < 2 ? 0 : kDP / 2 - 16) + 16 * fb + 8 * r4 + 4 * h;
+                const float4v value{st.o[fb][4 * r4], st.o[fb][4 * r4 + 1], st.o[fb][4 * r4 + 2], st.o[fb][4 * r4 + 3]};
+                if (feature < d)
+                    *reinterpret_cast<uint2v*>(row + feature) =
+                        uint2v{pack_pair<kBf16>(value[0] * inverse, value[1] * inverse),
+                               pack_pair<kBf16>(value[2] * inverse, value[3] * inverse)};
+            }
+    }
+}
+
+template <int DC>
+void launch_packed(const PackedParams& p, bool bf16, unsigned grid, hipStream_t stream) {
+    if (bf16)
+        packed_attention_kernel<DC, true><<<grid, kThreadsPerGroup, 0, stream>>>(p);
+    else
+        packed_attention_kernel<DC, false><<<grid, kThreadsPerGroup, 0, stream>>>(p);
+}
+
+}  // namespace
+}  // namespace tilemix
+
+extern "C" int tilemix_attention_packed(const TileMixPackedAttentionArgs* args, void* stream) {
+    using namespace tilemix;
+    if (!args) return hipErrorInvalidValue;
+    const TileMixPackedAttentionArgs& a = *args;
+    if (a.batch < 0 || a.q_tokens < 0 || a.k_tokens < 0 || a.q_heads <= 0 || a.kv_heads <= 0 || a.d <= 0 ||
+        a.q_heads % a.kv_heads != 0 || !std::isfinite(a.score_scale) ||
+        (a.dtype != TILEMIX_DTYPE_F16 && a.dtype != TILEMIX_DTYPE_BF16))
+        return hipErrorInvalidValue;
+    if (a.d > kMaxHeadDim) return hipErrorNotSupported;
+    if (a.d % 8 != 0) return hipErrorInvalidValue;
+    PackedParams p{};
+    Rows q, k, v, o;
+    if (!make_rows(q, a.Q, a.q_tokens, a.q_heads, a.d, a.q_row_stride, a.q_head_stride, 8) ||
+        !make_rows(k, a.K, a.k_tokens, a.kv_heads, a.d, a.k_row_stride, a.k_head_stride, 8) ||
+        !make_rows(v, a.V, a.k_tokens, a.kv_heads, a.d, a.v_row_stride, a.v_head_stride, 8) ||
+        !make_rows(o, a.O, a.q_tokens, a.q_heads, a.d, a.o_row_stride, a.o_head_stride, 4))
+        return hipErrorInvalidValue;
+    // A tile's rows are reached by 32-bit offsets.
+    constexpr std::int64_t kReach = (std::int64_t{1} << 30) / kTileKeys;
+    if (k.row > kReach || v.row > kReach) return hipErrorNotSupported;
+    if (a.batch == 0 || a.q_tokens == 0) return hipSuccess;
+    if (!a.q_starts) return hipErrorInvalidValue;
+    p.Q = a.Q;
+    p.K = a.K;
+    p.V = a.V;
+    p.O = a.O;
+    p.q_starts = a.q_starts;
+    p.k_starts = a.k_starts ? a.k_starts : a.q_starts;
+    p.q_row = q.row, p.q_head = q.head;
+    p.k_row = k.row, p.k_head = k.head;
+    p.v_row = v.row, p.v_head = v.head;
+    p.o_row = o.row, p.o_head = o.head;
+    p.batch = a.batch;
+    p.q_tokens = a.q_tokens;
+    p.k_tokens = a.k_tokens;
+    p.kv_heads = a.kv_heads;
+    p.group = a.q_heads / a.kv_heads;
+    p.team_shift = p.group % 4 == 0 ? 2 : p.group % 2 == 0 ? 1 : 0;
+    p.chunks = p.group >> p.team_shift;
+    p.d = a.d;
+    p.causal = a.causal != 0;
+    p.negate = a.score_scale < 0.0f;
+    p.score_log2 = std::fabs(a.score_scale) * kLog2e;
+    // Blocks of all sequences: each has at most one that is not full.
+    const int tokens = kBlockRows >> p.team_shift;
+    const std::int64_t blocks = a.q_tokens / tokens + static_cast<std::int64_t>(std::min(a.batch, a.q_tokens));
+    const std::int64_t grid = blocks * p.kv_heads * p.chunks;
+    if (grid > 0x7fffffffLL) return hipErrorInvalidConfiguration;
+    const hipError_t found = check_device();
+    if (found != hipSuccess) return found;
+    const bool bf16 = a.dtype == TILEMIX_DTYPE_BF16;
+    const hipStream_t s = static_cast<hipStream_t>(stream);
+    switch ((a.d + 31) / 32) {
+        case 1: launch_packed<1>(p, bf16, static_cast<unsigned>(grid), s); break;
+        case 2: launch_packed<2>(p, bf16, static_cast<unsigned>(grid), s); break;
+        case 3: launch_packed<3>(p, bf16, static_cast<unsigned>(grid), s); break;
+        default: launch_packed<4>(p, bf16, static_cast<unsigned>(grid), s); break;
+    }
+    return hipGetLastError();
+}

@@ -40,6 +40,10 @@ inline bool strided_heads_ok(int heads, int rows, int d, std::int64_t head_strid
     return head_stride >= d && static_cast<std::int64_t>(heads - 1) * head_stride + d <= row_stride;
 }
 
+// Whether the current device is one the kernels run on (hipErrorNotSupported
+// otherwise), and its compute units.
+hipError_t check_device(int* compute_units = nullptr);
+
 QuantSide make_quant_side(const std::uint16_t* x, std::int8_t* x8, std::uint16_t* scales,
                           std::int64_t head_stride, int rows, int block_rows, std::int64_t row_stride);
 

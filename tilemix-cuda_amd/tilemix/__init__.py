@@ -45,6 +45,19 @@ from .api import (  # noqa: F401
     SUCCESS,
     TileMixError,
 )
+from .serving import (  # noqa: F401
+    Cache4AppendArgs,
+    Cache4AttentionArgs,
+    Cache4GatherArgs,
+    PackedAttentionArgs,
+    attention_cache4,
+    attention_cache4_workspace_bytes,
+    attention_packed,
+    cache4_append,
+    cache4_block_bytes,
+    cache4_bytes,
+    cache4_gather,
+)
 from . import routing  # noqa: F401
 
 # Reference API constants (include/matmul_config.h:3-7, include/attention_fused.h:11-14).

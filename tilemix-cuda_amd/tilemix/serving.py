@@ -1,0 +1,202 @@
+"""Serving entry points of include/tilemix_capi.h: attention of packed sequences
+and the paged 4-bit key/value cache. Like the rest of the binding they take torch
+device tensors (or raw addresses, ``None`` for NULL) and return the hipError_t code;
+sizes, layouts and errors are those of the C header. Strides count elements, 0 =
+dense [tokens, heads, d].
+"""
+from __future__ import annotations
+
+import ctypes
+from dataclasses import dataclass
+from typing import Any
+
+from .api import _ptr, _stream, library
+
+_vp, _int, _i64, _sz, _f32 = ctypes.c_void_p, ctypes.c_int, ctypes.c_int64, ctypes.c_size_t, ctypes.c_float
+
+
+def _structure(name: str, fields: list[tuple[str, Any]]):
+    return type(name, (ctypes.Structure,), {"_fields_": fields})
+
+
+def _fields(pointers="", sizes="", int64s="") -> list[tuple[str, Any]]:
+    return ([(n, _vp) for n in pointers.split()] + [(n, _i64) for n in int64s.split()]
+            + [(n, _int) for n in sizes.split()])
+
+
+_PackedArgs = _structure("_PackedArgs", _fields(
+    "Q K V O q_starts k_starts", "batch q_tokens k_tokens q_heads kv_heads d dtype causal") + [("score_scale", _f32)]
+    + _fields(int64s="q_row_stride k_row_stride v_row_stride o_row_stride q_head_stride k_head_stride v_head_stride "
+                     "o_head_stride"))
+
+_AppendArgs = _structure("_AppendArgs", _fields("Q K V Q_out K_out cos_sin token_positions slots cache", int64s="pages")
+    + _fields(sizes="page_size tokens q_heads kv_heads d dtype rotary_dim interleaved positions")
+    + _fields(int64s="q_row_stride k_row_stride v_row_stride q_out_row_stride k_out_row_stride q_head_stride "
+                     "k_head_stride v_head_stride q_out_head_stride k_out_head_stride"))
+
+_GatherArgs = _structure("_GatherArgs", _fields("cache slots K_out V_out", int64s="pages")
+    + _fields(sizes="page_size tokens kv_heads d dtype")
+    + _fields(int64s="k_row_stride v_row_stride k_head_stride v_head_stride"))
+
+_Cache4AttentionArgs = _structure("_Cache4AttentionArgs", _fields("Q O cache block_table lengths workspace")
+    + [("workspace_bytes", _sz)] + _fields(int64s="pages table_stride")
+    + _fields(sizes="page_size max_pages batch q_heads kv_heads d dtype") + [("score_scale", _f32)]
+    + _fields(int64s="q_row_stride o_row_stride q_head_stride o_head_stride"))
+
+
+def _fill(structure, args):
+    """The C structure of a dataclass with the same field names."""
+    out = structure()
+    for name, kind in structure._fields_:
+        value = getattr(args, name)
+        setattr(out, name, _ptr(value) if kind is _vp else float(value) if kind is _f32 else int(value))
+    return out
+
+
+def _call(name: str, structure, args, stream) -> int:
+    function = getattr(library(), name)
+    function.argtypes, function.restype = [ctypes.POINTER(structure), _vp], _int
+    return function(ctypes.byref(_fill(structure, args)), _stream(stream))
+
+
+@dataclass
+class PackedAttentionArgs:
+    """TileMixPackedAttentionArgs: `batch` packed sequences, starts int32 [batch + 1] device tensors."""
+    Q: Any
+    K: Any
+    V: Any
+    O: Any
+    q_starts: Any
+    batch: int
+    q_tokens: int
+    k_tokens: int
+    q_heads: int
+    kv_heads: int
+    d: int
+    dtype: int  # DTYPE_F16 or DTYPE_BF16
+    score_scale: float
+    causal: bool = True
+    k_starts: Any = None  # None: q_starts
+    q_row_stride: int = 0
+    k_row_stride: int = 0
+    v_row_stride: int = 0
+    o_row_stride: int = 0
+    q_head_stride: int = 0
+    k_head_stride: int = 0
+    v_head_stride: int = 0
+    o_head_stride: int = 0
+
+
+@dataclass
+class Cache4AppendArgs:
+    """TileMixCache4AppendArgs: rotate Q and K, write K and V to the cache at `slots` (int64 [tokens])."""
+    K: Any
+    V: Any
+    slots: Any
+    cache: Any
+    pages: int
+    page_size: int
+    tokens: int
+    kv_heads: int
+    d: int
+    dtype: int
+    Q: Any = None
+    Q_out: Any = None
+    q_heads: int = 0
+    K_out: Any = None
+    cos_sin: Any = None  # fp32 [positions, rotary_dim]: cosines, then sines
+    token_positions: Any = None  # int32 [tokens]
+    positions: int = 0
+    rotary_dim: int = 0
+    interleaved: bool = False
+    q_row_stride: int = 0
+    k_row_stride: int = 0
+    v_row_stride: int = 0
+    q_out_row_stride: int = 0
+    k_out_row_stride: int = 0
+    q_head_stride: int = 0
+    k_head_stride: int = 0
+    v_head_stride: int = 0
+    q_out_head_stride: int = 0
+    k_out_head_stride: int = 0
+
+
+@dataclass
+class Cache4GatherArgs:
+    """TileMixCache4GatherArgs: cached rows at `slots` (int64 [tokens]) back in 16 bits."""
+    cache: Any
+    slots: Any
+    pages: int
+    page_size: int
+    tokens: int
+    kv_heads: int
+    d: int
+    dtype: int
+    K_out: Any = None
+    V_out: Any = None
+    k_row_stride: int = 0
+    v_row_stride: int = 0
+    k_head_stride: int = 0
+    v_head_stride: int = 0
+
+
+@dataclass
+class Cache4AttentionArgs:
+    """TileMixCache4AttentionArgs: one query token per sequence over its pages (block_table int32
+    [batch, max_pages], lengths int32 [batch]); `workspace` was set to zero once."""
+    Q: Any
+    O: Any
+    cache: Any
+    block_table: Any
+    lengths: Any
+    workspace: Any
+    workspace_bytes: int
+    pages: int
+    page_size: int
+    max_pages: int
+    batch: int
+    q_heads: int
+    kv_heads: int
+    d: int
+    dtype: int
+    score_scale: float
+    table_stride: int = 0  # 0: max_pages
+    q_row_stride: int = 0
+    o_row_stride: int = 0
+    q_head_stride: int = 0
+    o_head_stride: int = 0
+
+
+def attention_packed(args: PackedAttentionArgs, stream=None) -> int:
+    return _call("tilemix_attention_packed", _PackedArgs, args, stream)
+
+
+def cache4_append(args: Cache4AppendArgs, stream=None) -> int:
+    return _call("tilemix_cache4_append", _AppendArgs, args, stream)
+
+
+def cache4_gather(args: Cache4GatherArgs, stream=None) -> int:
+    return _call("tilemix_cache4_gather", _GatherArgs, args, stream)
+
+
+def attention_cache4(args: Cache4AttentionArgs, stream=None) -> int:
+    return _call("tilemix_attention_cache4", _Cache4AttentionArgs, args, stream)
+
+
+def cache4_block_bytes(d: int) -> int:
+    """Bytes of 32 tokens of one key head; 0 for a head dimension that is not supported."""
+    function = library().tilemix_cache4_block_bytes
+    function.argtypes, function.restype = [_int], _sz
+    return int(function(d))
+
+
+def cache4_bytes(pages: int, page_size: int, kv_heads: int, d: int) -> int:
+    function = library().tilemix_cache4_bytes
+    function.argtypes, function.restype = [_i64, _int, _int, _int], _sz
+    return int(function(pages, page_size, kv_heads, d))
+
+
+def attention_cache4_workspace_bytes() -> int:
+    function = library().tilemix_attention_cache4_workspace_bytes
+    function.argtypes, function.restype = [], _sz
+    return int(function())
