@@ -324,7 +324,7 @@ int tilemix_attention_packed(const TileMixPackedAttentionArgs* args, void* strea
  * (the last group possibly fewer) share a scale and a minimum, bf16 both, beside
  * their 4-bit codes: 4.5 bits a value for d of 64 or 128 (rows of other d take
  * the room of the next of these two). x is held as minimum + scale * code with
- *   minimum = bf16(least x), scale = bf16((largest x - minimum) / 15),
+ *   minimum = bf16(least x) (a zero positive), scale = bf16((largest x - minimum) / 15),
  *   code = clamp(round_half_even((x - minimum) / scale), 0, 15),
  * 0 where scale is below 2^-100; a group with an infinite or NaN value (or
  * a range past fp32's) is held as NaN. Order inside a block, with B = ceil(d / 64):

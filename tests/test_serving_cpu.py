@@ -1,0 +1,148 @@
+"""The serving entry points without a GPU: sizes of the cache, argument errors (all
+reported before any HIP runtime call), and the ctypes structures against the header."""
+from __future__ import annotations
+
+import ctypes
+import re
+from pathlib import Path
+
+import numpy as np
+import pytest
+
+import tilemix
+from tilemix import api, serving
+
+HEADER = Path(__file__).resolve().parent.parent / "include" / "tilemix_capi.h"
+INVALID, NOT_SUPPORTED = api.ERROR_INVALID_VALUE, api.ERROR_NOT_SUPPORTED
+NAN, INF = float("nan"), float("inf")
+
+_memory = np.zeros(64, dtype=np.uint8)
+X = (_memory.ctypes.data + 15) // 16 * 16  # a 16-byte aligned host address, never read
+
+
+def packed(**options):
+    return tilemix.PackedAttentionArgs(**{**dict(Q=X, K=X, V=X, O=X, q_starts=X, k_starts=X, batch=2, q_tokens=5, k_tokens=7,
+                                                 q_heads=4, kv_heads=2, d=64, dtype=tilemix.DTYPE_F16, score_scale=1.0), **options})
+
+
+def append(**options):
+    return tilemix.Cache4AppendArgs(**{**dict(
+        Q=X, K=X, V=X, Q_out=X, K_out=X, slots=X, cache=X, cos_sin=X, token_positions=X, positions=9, rotary_dim=64, pages=3,
+        page_size=32, tokens=5, q_heads=4, kv_heads=2, d=64, dtype=tilemix.DTYPE_BF16), **options})
+
+
+def gather(**options):
+    return tilemix.Cache4GatherArgs(**{**dict(cache=X, slots=X, K_out=X, V_out=X, pages=3, page_size=32, tokens=5, kv_heads=2,
+                                              d=64, dtype=tilemix.DTYPE_F16), **options})
+
+
+def decode(**options):
+    return tilemix.Cache4AttentionArgs(**{**dict(
+        Q=X, O=X, cache=X, block_table=X, lengths=X, workspace=X,
+        workspace_bytes=tilemix.attention_cache4_workspace_bytes(), pages=3, page_size=64, max_pages=2, batch=2, q_heads=4,
+        kv_heads=2, d=64, dtype=tilemix.DTYPE_F16, score_scale=1.0), **options})
+
+
+CALLS = {"packed": (tilemix.attention_packed, packed), "append": (tilemix.cache4_append, append),
+         "gather": (tilemix.cache4_gather, gather), "decode": (tilemix.attention_cache4, decode)}
+
+
+def code(kind, **options):
+    call, args = CALLS[kind]
+    return call(args(**options))
+
+
+def test_cache_sizes(tm):
+    # 32 tokens: codes of 64 or 128 features for keys and values, a scale and a minimum per 64.
+    for d in (8, 40, 64):
+        assert tm.cache4_block_bytes(d) == 32 * (32 + 32 + 4 + 4)
+    for d in (72, 96, 128):
+        assert tm.cache4_block_bytes(d) == 32 * (64 + 64 + 8 + 8)
+    for d in (0, -8, 4, 100, 129, 136):
+        assert tm.cache4_block_bytes(d) == 0
+    assert tm.cache4_bytes(10, 64, 8, 128) == 10 * 2 * 8 * 4608
+    assert tm.cache4_bytes(1 << 20, 256, 8, 128) == (1 << 20) * 8 * 8 * 4608  # past 2^32
+    for pages, page_size, heads, d in ((0, 32, 1, 64), (1, 0, 1, 64), (1, 33, 1, 64), (1, 16, 1, 64), (1, 32, 0, 64),
+                                       (1, 32, 1, 12), (-1, 32, 1, 64), (1 << 31, 32, 1, 64)):
+        assert tm.cache4_bytes(pages, page_size, heads, d) == 0
+    assert 0 < tm.attention_cache4_workspace_bytes() <= 16 << 20
+
+
+@pytest.mark.parametrize("kind", CALLS)
+def test_null_arguments(tm, kind):
+    assert getattr(tm.library(), {"packed": "tilemix_attention_packed", "append": "tilemix_cache4_append",
+                                  "gather": "tilemix_cache4_gather", "decode": "tilemix_attention_cache4"}[kind])(None, None) == INVALID
+    required = {"packed": "Q K V O q_starts", "append": "K V slots cache cos_sin token_positions Q Q_out",
+                "gather": "cache slots", "decode": "Q O cache block_table lengths workspace"}[kind]
+    for name in required.split():
+        assert code(kind, **{name: None}) == INVALID, name
+    assert code("gather", K_out=None, V_out=None) == INVALID
+
+
+@pytest.mark.parametrize("kind", CALLS)
+def test_sizes_types_and_alignment(tm, kind):
+    for d in (0, -8, 4, 60, 65, 127):
+        assert code(kind, d=d, **({"rotary_dim": 0} if kind == "append" else {})) == INVALID, d
+    for d in (129, 136, 2 ** 31 - 1):
+        assert code(kind, d=d) == NOT_SUPPORTED, d
+    for dtype in (tm.DTYPE_F32, 3, -1):
+        assert code(kind, dtype=dtype) == INVALID
+    assert code(kind, kv_heads=0) == INVALID and code(kind, kv_heads=-1) == INVALID
+    if kind in ("packed", "decode"):
+        assert code(kind, kv_heads=3) == INVALID and code(kind, q_heads=0) == INVALID
+        assert code(kind, batch=-1) == INVALID
+        for scale in (NAN, INF, -INF):
+            assert code(kind, score_scale=scale) == INVALID
+        assert code(kind, O=X + 4) == INVALID and code(kind, o_row_stride=4 * 64 + 2) == INVALID
+    if kind in ("append", "gather"):
+        assert code(kind, tokens=-1) == INVALID
+    if kind != "packed":
+        for bad in (dict(pages=0), dict(pages=-1), dict(pages=1 << 31), dict(page_size=0), dict(page_size=16),
+                    dict(page_size=48), dict(page_size=-32), dict(cache=X + 8)):
+            assert code(kind, **bad) == INVALID, bad
+    tensors = {"packed": {"q": "Q", "k": "K", "v": "V"}, "append": {"q": "Q", "k": "K", "v": "V", "q_out": "Q_out", "k_out": "K_out"},
+               "gather": {"k": "K_out", "v": "V_out"}, "decode": {"q": "Q"}}[kind]
+    for name, tensor in tensors.items():
+        heads = 2 if tensor[0] in "KV" else 4
+        assert code(kind, **{tensor: X + 8}) == INVALID, tensor                                  # 16-byte rows
+        assert code(kind, **{f"{name}_row_stride": heads * 64 + 4}) == INVALID, name             # whole pieces
+        assert code(kind, **{f"{name}_row_stride": heads * 64 - 8}) == INVALID, name             # rows overlap
+        assert code(kind, **{f"{name}_head_stride": 56}) == INVALID, name                        # heads overlap
+        assert code(kind, **{f"{name}_row_stride": -heads * 64}) == INVALID, name
+        assert code(kind, **{f"{name}_head_stride": -64}) == INVALID, name
+        assert code(kind, **{f"{name}_row_stride": 1 << 41}) == INVALID, name
+
+
+def test_refusals_of_one_operator(tm):
+    for rotary in (-2, 3, 66, 128):
+        assert code("append", rotary_dim=rotary) == INVALID
+    assert code("append", positions=0) == INVALID and code("append", q_heads=0) == INVALID
+    assert code("decode", max_pages=0) == INVALID and code("decode", table_stride=1) == INVALID
+    assert code("decode", table_stride=-2) == INVALID
+    assert code("decode", workspace=X + 4) == INVALID
+    assert code("decode", workspace_bytes=tm.attention_cache4_workspace_bytes() - 1) == INVALID
+    for stride in ("k_row_stride", "v_row_stride"):
+        assert code("packed", **{stride: (1 << 24) + 8}) == NOT_SUPPORTED
+    assert code("packed", q_tokens=-1) == INVALID and code("packed", k_tokens=-1) == INVALID
+
+
+def test_calls_with_nothing_to_do(tm):
+    """No device is asked for: they succeed on a machine without a GPU."""
+    assert code("packed", batch=0) == 0 and code("packed", q_tokens=0, Q=None, O=None) == 0
+    assert code("append", tokens=0, K=None, V=None, Q=None, Q_out=None, K_out=None, slots=None) == 0
+    assert code("gather", tokens=0, K_out=None, V_out=None, slots=None) == 0
+    assert code("decode", batch=0, Q=None, O=None, block_table=None, lengths=None) == 0
+
+
+def test_structures_match_the_header():
+    text = HEADER.read_text()
+    for structure, name in ((serving._PackedArgs, "TileMixPackedAttentionArgs"), (serving._AppendArgs, "TileMixCache4AppendArgs"),
+                            (serving._GatherArgs, "TileMixCache4GatherArgs"), (serving._Cache4AttentionArgs, "TileMixCache4AttentionArgs")):
+        body = re.search(r"typedef struct %s \{(.*?)\}" % name, text, re.S).group(1)
+        body = re.sub(r"/\*.*?\*/", "", body, flags=re.S)
+        kinds = {"int": ctypes.c_int, "float": ctypes.c_float, "int64_t": ctypes.c_int64, "size_t": ctypes.c_size_t}
+        fields = []
+        for line in filter(None, (x.strip() for x in body.split(";"))):
+            kind, field = line.rsplit(None, 1) if "*" not in line else ("pointer", line.split("*")[1].strip())
+            fields.append((field, ctypes.c_void_p if kind == "pointer" else kinds[kind]))
+        assert [tuple(f) for f in structure._fields_] == fields, name

@@ -215,7 +215,7 @@ __global__ __launch_bounds__(kCacheThreads) void cache4_append_kernel(const Appe
         low = over_8_lanes(low, [](float a, float b) { return fminf(a, b); });
         high = over_8_lanes(high, [](float a, float b) { return fmaxf(a, b); });
         zero = over_8_lanes(zero, [](float a, float b) { return a + b; });
-        const float minimum = half_of<true, 1>(pack_pair<true>(0.0f, low));
+        const float minimum = half_of<true, 1>(pack_pair<true>(0.0f, low)) + 0.0f;  // a zero without its sign
         std::uint32_t params = pack_pair<true>((high - minimum) / 15.0f, minimum);
         const float scale = half_of<true, 0>(params);
         const bool finite = zero == 0.0f && scale < INFINITY;
