@@ -26,6 +26,7 @@
 #include "tilemix_capi.h"
 
 #include <algorithm>
+#include <cfloat>
 #include <cmath>
 #include <type_traits>
 
@@ -73,24 +74,31 @@ __device__ __forceinline__ float4v mfma_16x16x32(uint4v a, uint4v b, float4v c) 
 }
 
 // 16 + code of the nibbles j of a word's halves, as a pair of fp16 (mantissa bits
-// 9 .. 6 under exponent 4) or bf16 (bits 6 .. 3).
-template <bool kBf16, int j>
-__device__ __forceinline__ std::uint32_t codes(std::uint32_t word) {
-    constexpr int kUp = (kBf16 ? 3 : 6) - 4 * j;
-    constexpr std::uint32_t kMask = kBf16 ? 0x00780078u : 0x03c003c0u, kSixteen = kBf16 ? 0x41804180u : 0x4c004c00u;
-    if constexpr (kUp >= 0)
-        return ((word << kUp) & kMask) | kSixteen;
-    else
-        return ((word >> -kUp) & kMask) | kSixteen;
-}
+// 9 .. 6 under exponent 4) or bf16 (bits 6 .. 3): two instructions, the second
+// written out, as the compiler, given two constants, makes it an and and an or.
 template <bool kBf16>
-__device__ __forceinline__ uint4v codes8(std::uint32_t word) {
-    return uint4v{codes<kBf16, 0>(word), codes<kBf16, 1>(word), codes<kBf16, 2>(word), codes<kBf16, 3>(word)};
-}
-template <int j>
-__device__ __forceinline__ uint4v codes_of(uint4v words) {  // nibble j of four words
-    return uint4v{codes<true, j>(words[0]), codes<true, j>(words[1]), codes<true, j>(words[2]), codes<true, j>(words[3])};
-}
+struct Codes {
+    std::uint32_t mask;  // in a vector register: an instruction takes one scalar
+    __device__ __forceinline__ Codes() {
+        if constexpr (kBf16) asm("v_mov_b32 %0, 0x00780078" : "=v"(mask));
+        else asm("v_mov_b32 %0, 0x03c003c0" : "=v"(mask));
+    }
+    template <int j>
+    __device__ __forceinline__ std::uint32_t pair(std::uint32_t word) const {
+        constexpr int kUp = (kBf16 ? 3 : 6) - 4 * j;
+        const std::uint32_t shifted = kUp >= 0 ? word << (kUp & 31) : word >> (-kUp & 31);
+        std::uint32_t out;
+        asm("v_and_or_b32 %0, %1, %2, %3" : "=v"(out) : "v"(shifted), "v"(mask), "s"(kBf16 ? 0x41804180u : 0x4c004c00u));
+        return out;
+    }
+    __device__ __forceinline__ uint4v all(std::uint32_t word) const {  // the word's 8 codes
+        return uint4v{pair<0>(word), pair<1>(word), pair<2>(word), pair<3>(word)};
+    }
+    template <int j>
+    __device__ __forceinline__ uint4v of(uint4v words) const {  // nibbles j of four words
+        return uint4v{pair<j>(words[0]), pair<j>(words[1]), pair<j>(words[2]), pair<j>(words[3])};
+    }
+};
 
 // Sum / maximum over the four lanes r, r + 16, r + 32, r + 48, in each of them.
 __device__ __forceinline__ void permlane16_swap(float& a, float& b) {
@@ -181,6 +189,7 @@ struct Block {
     std::uint32_t k[2][2 * kGroups];
     uint4v v[kGroups];
     uint4v k_params[kGroups][2], v_params[kGroups][2];
+    std::uint32_t row_params[2][kGroups];  // of token 16 b + r
 };
 
 template <int kGroups, bool kBf16>
@@ -255,6 +264,8 @@ __global__ __launch_bounds__(kThreads, 2) void cache4_attention_kernel(const Dec
                 const int at = 128 * m + 32 * g + 16 * x;
                 block.k_params[m][x] = __builtin_amdgcn_raw_buffer_load_b128(rs, cache_key_params_at(kGroups) + at, 0, 0);
                 block.v_params[m][x] = __builtin_amdgcn_raw_buffer_load_b128(rs, cache_value_params_at(kGroups) + at, 0, 0);
+                block.row_params[x][m] = __builtin_amdgcn_raw_buffer_load_b32(
+                    rs, cache_key_params_at(kGroups) + 128 * m + 4 * (8 * (r >> 2) + 4 * x + (r & 3)), 0, 0);
             }
     };
 
@@ -289,12 +300,29 @@ __global__ __launch_bounds__(kThreads, 2) void cache4_attention_kernel(const Dec
         }
         q_sum[m] = groups_sum(q_sum[m]);
     }
+    // B operand against (scale, minimum) words: 0, then sum q in three bf16 parts
+    // (all of its 24 bits), the first two in the lanes of group 0, the third in those of 1.
+    uint4v q_sums{0u, 0u, 0u, 0u};
+#pragma unroll
+    for (int m = 0; m < kGroups; ++m) {
+        const std::uint32_t first = pack_pair<true>(0.0f, q_sum[m]);
+        const float rest = q_sum[m] - half_of<true, 1>(first);
+        const std::uint32_t second = pack_pair<true>(0.0f, rest);
+        const std::uint32_t third = pack_pair<true>(0.0f, rest - half_of<true, 1>(second));
+        q_sums[m] = g == 0 ? first : g == 1 ? third : 0u;
+        q_sums[kGroups + m] = g == 0 ? second : 0u;
+    }
+    const Codes<kBf16> key_codes;
+    const Codes<true> value_codes;
+    const uint4v ones{0x3f803f80u, 0x3f803f80u, 0x3f803f80u, 0x3f803f80u};
 
     float4v o[kGroups][4];  // o[m][f][i]: row r, feature 64 m + 16 g + 4 i + f
-    float below[kGroups];   // the lane's part of sum p (minimum - 16 scale)
+    float below[kGroups];     // the lane's part of sum p minimum
+    float4v sixteen[kGroups];  // sum p scale, as multiplied, in every element
 #pragma unroll
     for (int m = 0; m < kGroups; ++m) {
         below[m] = 0.0f;
+        sixteen[m] = float4v{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
         for (int f = 0; f < 4; ++f) o[m][f] = float4v{0.0f, 0.0f, 0.0f, 0.0f};
     }
@@ -302,34 +330,43 @@ __global__ __launch_bounds__(kThreads, 2) void cache4_attention_kernel(const Dec
 
     auto compute = [&](const Block<kGroups>& block, int at) __attribute__((always_inline)) {
         // Slot e of group g: token 16 (e / 4) + 4 g + e % 4 of the block.
-        float s[8];
+        float4v s[2];
 #pragma unroll
-        for (int e = 0; e < 8; ++e) s[e] = 0.0f;
+        for (int b = 0; b < 2; ++b) {
+            const auto& words = block.row_params[b];
+            const uint4v params = kGroups == 2 ? uint4v{words[0], words[kGroups - 1], words[0], words[kGroups - 1]}
+                                               : uint4v{words[0], words[0], 0u, 0u};
+            s[b] = mfma_16x16x32<true>(params, q_sums, float4v{0.0f, 0.0f, 0.0f, 0.0f});
 #pragma unroll
-        for (int m = 0; m < kGroups; ++m) {
-            const float start = -16.0f * q_sum[m];
-#pragma unroll
-            for (int b = 0; b < 2; ++b) {
+            for (int m = 0; m < kGroups; ++m) {
+                const float start = -16.0f * q_sum[m];
                 float4v acc{start, start, start, start};
 #pragma unroll
-                for (int w = 0; w < 2; ++w)
-                    acc = mfma_16x16x32<kBf16>(codes8<kBf16>(block.k[b][2 * m + w]), qf[m][w], acc);
+                for (int w = 0; w < 2; ++w) acc = mfma_16x16x32<kBf16>(key_codes.all(block.k[b][2 * m + w]), qf[m][w], acc);
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const std::uint32_t params = block.k_params[m][b][i];
-                    s[4 * b + i] = __builtin_fmaf(half_of<true, 0>(params), acc[i],
-                                                  __builtin_fmaf(half_of<true, 1>(params), q_sum[m], s[4 * b + i]));
-                }
+                for (int i = 0; i < 4; ++i) s[b][i] = __builtin_fmaf(half_of<true, 0>(block.k_params[m][b][i]), acc[i], s[b][i]);
             }
         }
-        const int left = part.length - at * kCacheKeys;  // tokens from the block's first on
-        const bool tail = left < kCacheKeys;
+        uint4v v_params[kGroups][2];
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
-            s[e] *= p.score_log2;
-            if (tail && 16 * (e / 4) + 4 * g + e % 4 >= left) s[e] = -INFINITY;
+        for (int m = 0; m < kGroups; ++m)
+#pragma unroll
+            for (int x = 0; x < 2; ++x) v_params[m][x] = block.v_params[m][x];
+        const int left = part.length - at * kCacheKeys;  // tokens from the block's first on
+        if (left < kCacheKeys) {
+            // Past the length the block may hold anything, NaN included.
+            int mine = left - 4 * g;
+            asm volatile("" : "+v"(mine));  // a branch: one block in a sequence takes it
+#pragma unroll
+            for (int e = 0; e < 8; ++e)
+                if (16 * (e / 4) + e % 4 >= mine) {
+                    s[e / 4][e % 4] = -INFINITY;
+#pragma unroll
+                    for (int m = 0; m < kGroups; ++m) v_params[m][e / 4][e % 4] = 0u;
+                }
         }
-        const float top = max3(max3(s[0], s[1], s[2]), max3(s[3], s[4], s[5]), max3(s[6], s[7], s[7]));
+        const float c = p.score_log2;  // > 0
+        const float top = max3(max3(s[0][0], s[0][1], s[0][2]), max3(s[0][3], s[1][0], s[1][1]), max3(s[1][2], s[1][3], s[1][3])) * c;
         if (__any(top > row_max + kLazyRescale)) {
             const float m_new = fmaxf(row_max, groups_max(top));
             const float alpha = m_new == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(row_max - m_new);
@@ -337,6 +374,7 @@ __global__ __launch_bounds__(kThreads, 2) void cache4_attention_kernel(const Dec
 #pragma unroll
             for (int m = 0; m < kGroups; ++m) {
                 below[m] *= alpha;
+                sixteen[m] *= alpha;
 #pragma unroll
                 for (int f = 0; f < 4; ++f) o[m][f] *= alpha;
             }
@@ -346,7 +384,7 @@ __global__ __launch_bounds__(kThreads, 2) void cache4_attention_kernel(const Dec
         float prob[8];
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
-            prob[e] = __builtin_amdgcn_exp2f(s[e] + neg_m);
+            prob[e] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[e / 4][e % 4], c, neg_m));
             row_sum += prob[e];
         }
 #pragma unroll
@@ -358,26 +396,22 @@ __global__ __launch_bounds__(kThreads, 2) void cache4_attention_kernel(const Dec
 #pragma unroll
                 for (int x = 0; x < 2; ++x) {
                     const int e = 2 * t + x;
-                    std::uint32_t params = block.v_params[m][e / 4][e % 4];
-                    // Past the length the block may hold anything, NaN included.
-                    if (tail && 16 * (e / 4) + 4 * g + e % 4 >= left) params = 0u;
-                    const float scale = half_of<true, 0>(params);
-                    scaled[x] = prob[e] * scale;
-                    below[m] = __builtin_fmaf(prob[e], __builtin_fmaf(-16.0f, scale, half_of<true, 1>(params)), below[m]);
+                    const std::uint32_t params = v_params[m][e / 4][e % 4];
+                    scaled[x] = prob[e] * half_of<true, 0>(params);
+                    below[m] = __builtin_fmaf(prob[e], half_of<true, 1>(params), below[m]);
                 }
                 high[t] = pack_pair<true>(scaled[0], scaled[1]);
                 low[t] = pack_pair<true>(scaled[0] - half_of<true, 0>(high[t]), scaled[1] - half_of<true, 1>(high[t]));
             }
-            const uint4v a0 = codes_of<0>(block.v[m]), a1 = codes_of<1>(block.v[m]), a2 = codes_of<2>(block.v[m]),
-                         a3 = codes_of<3>(block.v[m]);
-            o[m][0] = mfma_16x16x32<true>(a0, high, o[m][0]);
-            o[m][1] = mfma_16x16x32<true>(a1, high, o[m][1]);
-            o[m][2] = mfma_16x16x32<true>(a2, high, o[m][2]);
-            o[m][3] = mfma_16x16x32<true>(a3, high, o[m][3]);
-            o[m][0] = mfma_16x16x32<true>(a0, low, o[m][0]);
-            o[m][1] = mfma_16x16x32<true>(a1, low, o[m][1]);
-            o[m][2] = mfma_16x16x32<true>(a2, low, o[m][2]);
-            o[m][3] = mfma_16x16x32<true>(a3, low, o[m][3]);
+            const uint4v a0 = value_codes.template of<0>(block.v[m]), a1 = value_codes.template of<1>(block.v[m]),
+                         a2 = value_codes.template of<2>(block.v[m]), a3 = value_codes.template of<3>(block.v[m]);
+            for (const uint4v& part_of_p : {high, low}) {
+                o[m][0] = mfma_16x16x32<true>(a0, part_of_p, o[m][0]);
+                o[m][1] = mfma_16x16x32<true>(a1, part_of_p, o[m][1]);
+                o[m][2] = mfma_16x16x32<true>(a2, part_of_p, o[m][2]);
+                o[m][3] = mfma_16x16x32<true>(a3, part_of_p, o[m][3]);
+                sixteen[m] = mfma_16x16x32<true>(ones, part_of_p, sixteen[m]);
+            }
         }
     };
     // Two blocks a turn, each loading the other's before it is computed; every wave
@@ -406,7 +440,7 @@ __global__ __launch_bounds__(kThreads, 2) void cache4_attention_kernel(const Dec
     }
 #pragma unroll
     for (int m = 0; m < kGroups; ++m) {
-        const float rest = groups_sum(below[m]);
+        const float rest = __builtin_fmaf(-16.0f, sixteen[m][0], groups_sum(below[m]));
 #pragma unroll
         for (int i = 0; i < 4; ++i)
             *reinterpret_cast<float4v*>(&lds_o[wave][r][64 * m + 16 * g + 4 * i]) =
@@ -522,7 +556,8 @@ extern "C" int tilemix_attention_cache4(const TileMixCache4AttentionArgs* args, 
     // A multiple of 32 under 2^31, so that block counts do not overflow.
     p.most_tokens = static_cast<int>(std::min<std::int64_t>(static_cast<std::int64_t>(a.max_pages) * a.page_size, 0x7fffffe0LL));
     p.negate = a.score_scale < 0.0f;
-    p.score_log2 = std::fabs(a.score_scale) * kLog2e;
+    // (Of a score_scale of 0 the smallest number: a hidden token's -inf times it is still -inf.)
+    p.score_log2 = std::max(std::fabs(a.score_scale) * kLog2e, FLT_MIN);
     // The parts wanted, and one more per sequence, head and tile whose last part is not whole.
     const std::int64_t heads = static_cast<std::int64_t>(a.kv_heads) * p.tiles;
     const std::int64_t most = (p.most_tokens / kCacheKeys + kLeastSteps - 1) / kLeastSteps;  // of one of them

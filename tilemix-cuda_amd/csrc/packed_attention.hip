@@ -30,7 +30,8 @@
 namespace tilemix {
 namespace {
 
-constexpr int kBlockRows = 128;  // query rows (tokens x heads) of a workgroup
+constexpr int kBlockShift = 7;
+constexpr int kBlockRows = 1 << kBlockShift;  // query rows (tokens x heads) of a workgroup
 
 struct PackedParams {
     const std::uint16_t* Q;
@@ -84,26 +85,27 @@ __device__ __forceinline__ int wave_sum(int v) {
     return __builtin_amdgcn_readfirstlane(a + b);
 }
 
-// Blocks of `tokens` query tokens of a sequence that walk at least `tiles` key tiles.
-__device__ __forceinline__ int blocks_walking(const Sequence& s, int tokens, int tiles, bool causal) {
-    const int blocks = (s.q_len + tokens - 1) / tokens;
+// Blocks of 1 << shift query tokens of a sequence that walk at least `tiles` key tiles.
+__device__ __forceinline__ int blocks_walking(const Sequence& s, int shift, int tiles, bool causal) {
+    const int blocks = static_cast<int>((static_cast<unsigned>(s.q_len) + (1u << shift) - 1) >> shift);
     if (tiles <= 0) return blocks;
-    const std::int64_t keys = std::int64_t{kTileKeys} * (tiles - 1) + 1;  // the fewest of so many tiles
-    if (s.k_len < keys) return 0;
+    // More than `hidden` keys are as many tiles; k_len and the rows are under 2^31, a tile count under 2^25.
+    const unsigned hidden = static_cast<unsigned>(kTileKeys) * static_cast<unsigned>(tiles - 1);
+    if (static_cast<unsigned>(s.k_len) <= hidden) return 0;
     if (!causal) return blocks;
-    // Block j sees keys up to k_len - q_len + (j + 1) tokens.
-    const std::int64_t first = (keys - (s.k_len - s.q_len) + tokens - 1) / tokens - 1;
-    return first <= 0 ? blocks : static_cast<int>(first < blocks ? blocks - first : 0);
+    // Block j sees min(k_len, k_len - q_len + (j + 1 << shift)) keys: too few up to row `few`.
+    const int few = s.q_len - static_cast<int>(static_cast<unsigned>(s.k_len) - hidden);
+    return blocks - (max(few, 0) >> shift);
 }
 
 // The sequence and block of work item `slot`, items of more key tiles first
 // (the last to start are the shortest; a long walk that starts last would run
 // alone); false past the last. Wave-uniform.
-__device__ __forceinline__ bool find_block(const PackedParams& p, int slot, int tokens, int lane, Sequence& found, int& block) {
+__device__ __forceinline__ bool find_block(const PackedParams& p, int slot, int shift, int lane, Sequence& found, int& block) {
     const bool causal = p.causal != 0;
     if (p.batch == 1) {
         found = sequence_at(p, 0);
-        const int blocks = (found.q_len + tokens - 1) / tokens;
+        const int blocks = blocks_walking(found, shift, 0, causal);
         block = blocks - 1 - slot;
         return slot < blocks;
     }
@@ -111,9 +113,9 @@ __device__ __forceinline__ bool find_block(const PackedParams& p, int slot, int 
     if (lane < p.batch) mine = sequence_at(p, lane);
     const bool few = p.batch <= kWave;
     auto count = [&](int tiles) {
-        int n = blocks_walking(mine, tokens, tiles, causal);
+        int n = blocks_walking(mine, shift, tiles, causal);
         if (!few)
-            for (int b = lane + kWave; b < p.batch; b += kWave) n += blocks_walking(sequence_at(p, b), tokens, tiles, causal);
+            for (int b = lane + kWave; b < p.batch; b += kWave) n += blocks_walking(sequence_at(p, b), shift, tiles, causal);
         return wave_sum(n);
     };
     if (count(0) <= slot) return false;
@@ -131,8 +133,8 @@ __device__ __forceinline__ bool find_block(const PackedParams& p, int slot, int 
         const int b = base + lane;
         Sequence s{0, 0, 0, 0};
         if (b < p.batch) s = sequence_at(p, b);
-        const int above = blocks_walking(s, tokens, low + 1, causal);
-        const int here = blocks_walking(s, tokens, low, causal) - above;
+        const int above = blocks_walking(s, shift, low + 1, causal);
+        const int here = blocks_walking(s, shift, low, causal) - above;
         int before = here;  // inclusive prefix over the lanes
 #pragma unroll
         for (int step = 1; step < kWave; step <<= 1) {
@@ -147,7 +149,7 @@ __device__ __forceinline__ bool find_block(const PackedParams& p, int slot, int 
             found.k0 = __builtin_amdgcn_readlane(s.k0, at);
             found.k_len = __builtin_amdgcn_readlane(s.k_len, at);
             // Blocks of a sequence walk more tiles the later they are.
-            const int blocks = (found.q_len + tokens - 1) / tokens;
+            const int blocks = blocks_walking(found, shift, 0, causal);
             block = blocks - 1 - __builtin_amdgcn_readlane(above, at) - (rest - __builtin_amdgcn_readlane(before - here, at));
             return true;
         }
@@ -272,7 +274,7 @@ __global__ __launch_bounds__(kThreadsPerGroup, 2) void packed_attention_kernel(c
     const int tokens = kBlockRows >> p.team_shift;
     Sequence seq;
     int block;
-    if (!find_block(p, slot, tokens, lane, seq, block)) return;
+    if (!find_block(p, slot, kBlockShift - p.team_shift, lane, seq, block)) return;
     const int context = seq.k_len - seq.q_len;  // row i sees keys up to context + i
     const int head = kv_head * p.group + (chunk << p.team_shift) + (wave & (team_heads - 1));
     const int t0 = block * tokens;
