@@ -39,11 +39,12 @@ namespace {
 
 constexpr int kWaves = 4;
 constexpr int kThreads = kWaves * kWave;
-constexpr int kGroupsPerUnit = 2;  // workgroups of a CU that registers are allocated for
-constexpr int kSlots = 3;         // blocks in a wave's ring: one computed, two under way
+constexpr int kGroupsPerUnit = 3;  // workgroups of a CU that registers are allocated for
+constexpr int kSlots = 2;         // blocks in a wave's ring: one computed, the others under way
 constexpr int kTileRows = 16;     // query rows of a workgroup
 constexpr int kLeastSteps = 8;  // blocks of a range: two for each wave
-constexpr int kRanges = 512;    // at most: workgroups that the device holds at once
+constexpr int kRanges16 = 512;  // the same of the kernel with 16 rows, which takes more LDS
+constexpr int kRanges = 768;    // at most: workgroups that the device holds at once
 // The workspace: arrival counters, then rows of O and their states for the two parts
 // (one continued, one to be continued) that a range can have.
 constexpr std::size_t kWorkspaceBytes =
@@ -107,17 +108,9 @@ struct Codes {
     }
 };
 
-// Sum / maximum over the four lanes r, r + 16, r + 32, r + 48, in each of them.
+// Sum over the four lanes r, r + 16, r + 32, r + 48, in each of them.
 __device__ __forceinline__ void permlane16_swap(float& a, float& b) {
     asm volatile("s_nop 1\n\tv_permlane16_swap_b32 %0, %1" : "+v"(a), "+v"(b));
-}
-__device__ __forceinline__ float groups_max(float x) {
-    float a = x, b = x;
-    permlane16_swap(a, b);
-    a = fmaxf(a, b);
-    b = a;
-    permlane32_swap(a, b);
-    return fmaxf(a, b);
 }
 __device__ __forceinline__ float groups_sum(float x) {
     float a = x, b = x;
@@ -126,6 +119,19 @@ __device__ __forceinline__ float groups_sum(float x) {
     b = a;
     permlane32_swap(a, b);
     return a + b;
+}
+
+// f over the 16 lanes of a row, in each of them (DPP: quad partners, then mirrored).
+template <typename F>
+__device__ __forceinline__ float over_16_lanes(float x, F&& f) {
+    auto step = [&](auto control) __attribute__((always_inline)) {
+        constexpr int kControl = decltype(control)::value;
+        return __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, x), kControl, 0xf, 0xf, false));
+    };
+    x = f(x, step(std::integral_constant<int, 0xb1>{}));
+    x = f(x, step(std::integral_constant<int, 0x4e>{}));
+    x = f(x, step(std::integral_constant<int, 0x141>{}));
+    return f(x, step(std::integral_constant<int, 0x140>{}));
 }
 
 // Inclusive prefix sum over the lanes: DPP steps inside rows of 16 lanes, then the last
@@ -216,21 +222,42 @@ __device__ __forceinline__ void load_dwords_to_lds(int4v rsrc, unsigned lds_addr
                  : "memory");
 }
 
-template <int kGroups, bool kBf16>
+// kRows: query rows of a workgroup, 8 or 16. Scores are taken with queries as the rows
+// and tokens as the columns of a tile, so that a lane has 4 rows of a token (of two with
+// 16 rows), and its scale and minimum once; with 8 rows the two halves of a
+// tile are the same rows, and hold the two 16-token halves of a block.
+template <int kGroups, bool kBf16, int kRows>
 __global__ __launch_bounds__(kThreads, kGroupsPerUnit) void cache4_attention_kernel(const DecodeParams p) {
+    constexpr int kTiles = kRows / 8;  // tokens of a lane
     constexpr int kDP = 64 * kGroups;
     constexpr int kBlockBytes = cache_block_bytes(kGroups);
     constexpr int kLoads = 3 * kGroups;  // of a block: 2 kGroups KiB of codes, then 256-byte pieces of parameters
     __shared__ __attribute__((aligned(16))) unsigned char lds_blocks[kWaves][kSlots][kBlockBytes];  // a ring per wave
-    __shared__ __attribute__((aligned(16))) float lds_o[kWaves][kTileRows][kCacheGroup];
-    __shared__ float lds_ml[kWaves][kTileRows][2];
-    __shared__ int lds_last;
+    // A wave's piece: p scale on its way to the matrix operand's layout while blocks are computed,
+    // 32 features of O at a segment's end.
+    constexpr int kTurnBytes = kGroups * 2 * kRows * kCacheKeys * 2, kQuads = 8;
+    constexpr int kPieceBytes = kTurnBytes > kTileRows * kQuads * 16 ? kTurnBytes : kTileRows * kQuads * 16;
+    __shared__ __attribute__((aligned(16))) unsigned char lds_piece[kWaves][kPieceBytes];
+    __shared__ __attribute__((aligned(16))) float lds_ml[kWaves][kTileRows][4];  // maximum, sum, sum p minimum of both groups
+    __shared__ int lds_last[2];
 
     const int tid = threadIdx.x;
     const int lane = tid & (kWave - 1);
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int r = lane & 15;  // token of a score block / feature quarter (A operands), query row (B operands, results)
     const int g = lane >> 4;
+    // The lane's rows row0 .. + 3, its (first) token of a block and that token's place.
+    const int row0 = 4 * g % kRows, token0 = r + (kTiles == 1 ? 16 * (g >> 1) : 0), place0 = cache_place(token0);
+    // Over the lanes that hold the same rows.
+    auto row_reduce = [&](float x, auto&& f) __attribute__((always_inline)) {
+        x = over_16_lanes(x, f);
+        if constexpr (kTiles == 1) {
+            float y = x;
+            permlane32_swap(x, y);
+            x = f(x, y);
+        }
+        return x;
+    };
     Segment segment;
     std::int64_t range_length;
     const int range = blockIdx.x;
@@ -295,6 +322,17 @@ __global__ __launch_bounds__(kThreads, kGroupsPerUnit) void cache4_attention_ker
     int slot = 0;       // its place
     uint4v qf[kGroups][2];
     int rows = 0, head0 = 0;
+    Segment next;
+    bool more = true, next_window = false;
+    int next_page = 0;  // window of the wave's first pages of `next`
+    auto look_ahead = [&]() __attribute__((always_inline)) {
+        next = segment;
+        next_window = segment.end == segment.blocks && next_segment(p, next, range_end);
+        if (next_window) {
+            const int pages = (next.length + p.cache.page_size - 1) / p.cache.page_size, first = wave / per_page;
+            next_page = first + lane < pages ? p.table[next.sequence * p.table_stride + first + lane] : -1;
+        }
+    };
     // Queries and the wave's first blocks of `segment`, on their way.
     auto begin_segment = [&]() __attribute__((always_inline)) {
         const int head = segment.item / p.tiles, tile = segment.item - head * p.tiles;
@@ -305,15 +343,20 @@ __global__ __launch_bounds__(kThreads, kGroupsPerUnit) void cache4_attention_ker
         step = segment.first + wave;
         page = step / per_page;
         inside = step - page * per_page;
-        load_window();
+        if (next_window) {
+            window = page;
+            window_page = next_page;
+        } else {
+            load_window();
+        }
 #pragma unroll
         for (int m = 0; m < kGroups; ++m)
 #pragma unroll
             for (int w = 0; w < 2; ++w) {
                 const int feature = 64 * m + 16 * g + 8 * w;
                 qf[m][w] = uint4v{0u, 0u, 0u, 0u};
-                if (r < rows && feature < d)
-                    qf[m][w] = *reinterpret_cast<const uint4v*>(p.Q + segment.sequence * p.q.row + (head0 + r) * p.q.head + feature);
+                if (r % kRows < rows && feature < d)
+                    qf[m][w] = *reinterpret_cast<const uint4v*>(p.Q + segment.sequence * p.q.row + (head0 + r % kRows) * p.q.head + feature);
             }
         find();
         slot = 0;
@@ -328,149 +371,200 @@ __global__ __launch_bounds__(kThreads, kGroupsPerUnit) void cache4_attention_ker
     const Codes<kBf16> key_codes;
     const Codes<true> value_codes;
     const uint4v ones{0x3f803f80u, 0x3f803f80u, 0x3f803f80u, 0x3f803f80u};
+    // What the range has a part of, at most two: merged, where this workgroup is the last
+    // to arrive, at the end.
+    struct Shared {
+        int first_range, count, rows;
+        std::uint16_t* out;
+    };
+    Shared shared[2];
+    int shares = 0;
+    const int row = tid / kQuads, quad = tid % kQuads;  // a thread's row and 4 features in a pass of the merges
+    constexpr int kPasses = 2 * kGroups;
+    const int thread_feature = 16 * (quad >> 1) + 4 * (quad & 1);  // + 32 (pass / 2) * 2 + 8 (pass % 2)
+    auto feature_of = [&](int pass) __attribute__((always_inline)) { return 64 * (pass / 2) + 8 * (pass % 2) + thread_feature; };
+    auto store_rows = [&](const float4v (&value)[kPasses], float l, std::uint16_t* out) __attribute__((always_inline)) {
+        const float inverse = l == 0.0f ? 0.0f : 1.0f / l;  // 0: no token
+#pragma unroll
+        for (int x = 0; x < kPasses; ++x)
+            if (feature_of(x) < d)
+                *reinterpret_cast<uint2v*>(out + row * p.o.head + feature_of(x)) =
+                    uint2v{pack_pair<kBf16>(value[x][0] * inverse, value[x][1] * inverse),
+                           pack_pair<kBf16>(value[x][2] * inverse, value[x][3] * inverse)};
+    };
+    // Parts in the workspace: part i of a sequence and head is the continued one of range
+    // first_range + i, part 0 the one to be continued.
+    constexpr int kPartO = kTileRows * kDP, kPartMl = kTileRows * 2;
+    const Rsrc ro = shared_rows(p.part_o, std::int64_t{2} * kRanges * kPartO);
+    const Rsrc rml = shared_rows(p.part_ml, std::int64_t{2} * kRanges * kPartMl);
+    auto part_place = [](int first_range, int i) { return 2 * (first_range + i) + (i == 0 ? 1 : 0); };
+    auto part_at = [&](int place, int pass) __attribute__((always_inline)) {
+        return (place * kPartO + (pass * kTileRows + row) * (4 * kQuads) + 4 * quad) * 4;
+    };
     begin_segment();
-    for (bool more = true; more;) {
-    float q_sum[kGroups];  // of the row's features
+    while (more) {
+    look_ahead();
+    // q_sum[m][i]: of the features of row row0 + i.
+    float4v q_sum[kGroups];
 #pragma unroll
     for (int m = 0; m < kGroups; ++m) {
-        q_sum[m] = 0.0f;
+        float sum = 0.0f;  // of row r
 #pragma unroll
         for (int w = 0; w < 2; ++w) {
             if (p.negate) qf[m][w] ^= 0x80008000u;
 #pragma unroll
-            for (int x = 0; x < 4; ++x) q_sum[m] += half_of<kBf16, 0>(qf[m][w][x]) + half_of<kBf16, 1>(qf[m][w][x]);
+            for (int x = 0; x < 4; ++x) sum += half_of<kBf16, 0>(qf[m][w][x]) + half_of<kBf16, 1>(qf[m][w][x]);
         }
-        q_sum[m] = groups_sum(q_sum[m]);
-    }
-    // B operand against (scale, minimum) words: 0, then sum q in three bf16 parts
-    // (all of its 24 bits), the first two in the lanes of group 0, the third in those of 1.
-    uint4v q_sums{0u, 0u, 0u, 0u};
+        sum = groups_sum(sum);
 #pragma unroll
-    for (int m = 0; m < kGroups; ++m) {
-        const std::uint32_t first = pack_pair<true>(0.0f, q_sum[m]);
-        const float rest = q_sum[m] - half_of<true, 1>(first);
-        const std::uint32_t second = pack_pair<true>(0.0f, rest);
-        const std::uint32_t third = pack_pair<true>(0.0f, rest - half_of<true, 1>(second));
-        q_sums[m] = g == 0 ? first : g == 1 ? third : 0u;
-        q_sums[kGroups + m] = g == 0 ? second : 0u;
+        for (int i = 0; i < 4; ++i) q_sum[m][i] = __shfl(sum, row0 + i);
     }
 
-    float4v o[kGroups][4];  // o[m][f][i]: row r, feature 64 m + 16 g + 4 i + f
-    float below[kGroups];     // the lane's part of sum p minimum
-    float4v sixteen[kGroups];  // sum p scale, as multiplied, in every element
+    float4v o[kGroups][4];     // o[m][f][i]: column r, feature 64 m + 16 g + 4 i + f
+    float4v sixteen[kGroups];  // sum p scale, as multiplied, of column r in every element
+    float4v below[kGroups];    // of the lane's tokens: sum p minimum,
+    float4v row_sum{0.0f, 0.0f, 0.0f, 0.0f};  // and sum p,
+    float4v row_max{-INFINITY, -INFINITY, -INFINITY, -INFINITY};  // of the rows row0 + i
 #pragma unroll
     for (int m = 0; m < kGroups; ++m) {
-        below[m] = 0.0f;
-        sixteen[m] = float4v{0.0f, 0.0f, 0.0f, 0.0f};
+        below[m] = sixteen[m] = float4v{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
         for (int f = 0; f < 4; ++f) o[m][f] = float4v{0.0f, 0.0f, 0.0f, 0.0f};
     }
-    float row_max = -INFINITY, row_sum = 0.0f;  // row_sum: the lane's part
 
     auto compute = [&](int at_step) __attribute__((always_inline)) {
         const unsigned char* const block = &lds_blocks[wave][slot][0];
-        // Slot e of group g: token 16 (e / 4) + 4 g + e % 4 of the block, at place 8 g + e.
-        auto params_of = [&](int which, int m, int x) __attribute__((always_inline)) {
-            return *reinterpret_cast<const uint4v*>(block + cache_key_params_at(kGroups) + 128 * (which * kGroups + m) + 32 * g + 16 * x);
-        };
-        float4v s[2];
+        const int left = segment.length - at_step * kCacheKeys;  // tokens from the block's first on
+        float4v s[kTiles];       // rows row0 + i of the tile's token of the lane
+        std::uint32_t v_params[kTiles][kGroups];
+#pragma unroll
+        for (int t = 0; t < kTiles; ++t) s[t] = float4v{0.0f, 0.0f, 0.0f, 0.0f};
+        std::uint32_t k[2][2 * kGroups];  // codes of the lane's features of token 16 b + r
 #pragma unroll
         for (int b = 0; b < 2; ++b) {
-            std::uint32_t words[kGroups];  // of token 16 b + r
-#pragma unroll
-            for (int m = 0; m < kGroups; ++m)
-                words[m] = *reinterpret_cast<const std::uint32_t*>(block + cache_key_params_at(kGroups) + 128 * m +
-                                                                   4 * (8 * (r >> 2) + 4 * b + (r & 3)));
-            std::uint32_t k[2 * kGroups];  // codes of the lane's features of token 16 b + r
             if constexpr (kGroups == 2) {
                 const uint4v codes = *reinterpret_cast<const uint4v*>(block + 64 * (16 * b + r) + 16 * g);
 #pragma unroll
-                for (int w = 0; w < 4; ++w) k[w] = codes[w];
+                for (int w = 0; w < 4; ++w) k[b][w] = codes[w];
             } else {
                 const uint2v codes = *reinterpret_cast<const uint2v*>(block + 32 * (16 * b + r) + 8 * g);
-                k[0] = codes[0], k[1] = codes[1];
+                k[b][0] = codes[0], k[b][1] = codes[1];
             }
-            const uint4v params = kGroups == 2 ? uint4v{words[0], words[kGroups - 1], words[0], words[kGroups - 1]}
-                                               : uint4v{words[0], words[0], 0u, 0u};
-            s[b] = mfma_16x16x32<true>(params, q_sums, float4v{0.0f, 0.0f, 0.0f, 0.0f});
-#pragma unroll
-            for (int m = 0; m < kGroups; ++m) {
-                const float start = -16.0f * q_sum[m];
-                float4v acc{start, start, start, start};
-#pragma unroll
-                for (int w = 0; w < 2; ++w) acc = mfma_16x16x32<kBf16>(key_codes.all(k[2 * m + w]), qf[m][w], acc);
-                const uint4v scales = params_of(0, m, b);
-#pragma unroll
-                for (int i = 0; i < 4; ++i) s[b][i] = __builtin_fmaf(half_of<true, 0>(scales[i]), acc[i], s[b][i]);
-            }
-        }
-        // Past the length the block may hold anything, NaN included. The compiler must
-        // not turn these branches into selects: one block in a sequence takes them.
-        const int left = segment.length - at_step * kCacheKeys;  // tokens from the block's first on
-        if (left < kCacheKeys) {
-            int mine = left - 4 * g;
-            asm volatile("" : "+v"(mine));
-#pragma unroll
-            for (int e = 0; e < 8; ++e)
-                if (16 * (e / 4) + e % 4 >= mine) s[e / 4][e % 4] = -INFINITY;
-        }
-        const float c = p.score_log2;  // > 0
-        const float top = max3(max3(s[0][0], s[0][1], s[0][2]), max3(s[0][3], s[1][0], s[1][1]), max3(s[1][2], s[1][3], s[1][3])) * c;
-        if (__any(top > row_max + kLazyRescale)) {
-            const float m_new = fmaxf(row_max, groups_max(top));
-            const float alpha = m_new == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(row_max - m_new);
-            row_max = m_new;
-#pragma unroll
-            for (int m = 0; m < kGroups; ++m) {
-                below[m] *= alpha;
-                sixteen[m] *= alpha;
-#pragma unroll
-                for (int f = 0; f < 4; ++f) o[m][f] *= alpha;
-            }
-            row_sum *= alpha;
-        }
-        const float neg_m = row_max == -INFINITY ? 0.0f : -row_max;
-        float prob[8];
-#pragma unroll
-        for (int e = 0; e < 8; ++e) {
-            prob[e] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[e / 4][e % 4], c, neg_m));
-            row_sum += prob[e];
         }
 #pragma unroll
         for (int m = 0; m < kGroups; ++m) {
-            uint4v v_params[2] = {params_of(1, m, 0), params_of(1, m, 1)};
-            if (left < kCacheKeys) {
-                int mine = left - 4 * g;
-                asm volatile("" : "+v"(mine));
+            float4v acc[2];  // sum (16 + code) q of rows 4 g + i (mod kRows) and token 16 b + r
 #pragma unroll
-                for (int e = 0; e < 8; ++e)
-                    if (16 * (e / 4) + e % 4 >= mine) v_params[e / 4][e % 4] = 0u;
+            for (int b = 0; b < 2; ++b) {
+                acc[b] = float4v{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+                for (int w = 0; w < 2; ++w) acc[b] = mfma_16x16x32<kBf16>(qf[m][w], key_codes.all(k[b][2 * m + w]), acc[b]);
             }
-            uint4v high, low;
 #pragma unroll
-            for (int t = 0; t < 4; ++t) {
-                float scaled[2];
+            for (int t = 0; t < kTiles; ++t) {
+                const unsigned char* const params = block + 4 * place0 + 16 * t + 128 * m;
+                const std::uint32_t word = *reinterpret_cast<const std::uint32_t*>(params + cache_key_params_at(kGroups));
+                v_params[t][m] = *reinterpret_cast<const std::uint32_t*>(params + cache_value_params_at(kGroups));
+                const float scale = half_of<true, 0>(word), low = __builtin_fmaf(-16.0f, scale, half_of<true, 1>(word));
 #pragma unroll
-                for (int x = 0; x < 2; ++x) {
-                    const int e = 2 * t + x;
-                    const std::uint32_t params = v_params[e / 4][e % 4];
-                    scaled[x] = prob[e] * half_of<true, 0>(params);
-                    below[m] = __builtin_fmaf(prob[e], half_of<true, 1>(params), below[m]);
+                for (int i = 0; i < 4; ++i) {
+                    // With 8 rows the tile holds them twice: the lanes of the upper half take token 16 + r.
+                    const float sum = kTiles == 2 ? acc[t][i] : g >= 2 ? acc[1][i] : acc[0][i];
+                    s[t][i] = __builtin_fmaf(scale, sum, __builtin_fmaf(low, q_sum[m][i], s[t][i]));
                 }
-                high[t] = pack_pair<true>(scaled[0], scaled[1]);
-                low[t] = pack_pair<true>(scaled[0] - half_of<true, 0>(high[t]), scaled[1] - half_of<true, 1>(high[t]));
             }
+        }
+        // Past the length the block may hold anything, NaN included.
+#pragma unroll
+        for (int t = 0; t < kTiles; ++t)
+            if (token0 + 16 * t >= left) {
+                s[t] = float4v{-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+                for (int m = 0; m < kGroups; ++m) v_params[t][m] = 0u;
+            }
+        const float c = p.score_log2;  // > 0
+        float over = -INFINITY;  // how far a score is above its row's maximum
+#pragma unroll
+        for (int t = 0; t < kTiles; ++t)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                s[t][i] *= c;
+                over = fmaxf(over, s[t][i] - row_max[i]);
+            }
+        // (-inf - -inf is NaN, which fmaxf passes over: such a row stays as it is.)
+        if (__any(over > kLazyRescale)) {
+            float4v alpha;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const float top = row_reduce(kTiles == 2 ? fmaxf(s[0][i], s[kTiles - 1][i]) : s[0][i], [](float x, float y) { return fmaxf(x, y); });
+                const float m_new = fmaxf(row_max[i], top);
+                alpha[i] = m_new == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(row_max[i] - m_new);
+                row_max[i] = m_new;
+            }
+            row_sum *= alpha;
+            // The columns' factors, through LDS.
+            float* const factors = &lds_ml[wave][0][0];
+            if (r == 0 && (kTiles == 2 || g < 2)) *reinterpret_cast<float4v*>(factors + row0) = alpha;
+            asm volatile("" ::: "memory");
+            const float factor = factors[r % kRows];
+            asm volatile("" ::: "memory");
+#pragma unroll
+            for (int m = 0; m < kGroups; ++m) {
+                below[m] *= alpha;
+                sixteen[m] *= factor;
+#pragma unroll
+                for (int f = 0; f < 4; ++f) o[m][f] *= factor;
+            }
+        }
+        float4v prob[kTiles];
+#pragma unroll
+        for (int t = 0; t < kTiles; ++t)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                prob[t][i] = __builtin_amdgcn_exp2f(s[t][i] - (row_max[i] == -INFINITY ? 0.0f : row_max[i]));
+                row_sum[i] += prob[t][i];
+            }
+        // p scale in two bf16 parts, from tokens in lanes and rows in registers to the
+        // matrix operand's columns: [m][part][row][place] in the wave's piece.
+        std::uint16_t* const turn = reinterpret_cast<std::uint16_t*>(lds_piece[wave]);
+        asm volatile("" ::: "memory");
+#pragma unroll
+        for (int m = 0; m < kGroups; ++m)
+#pragma unroll
+            for (int t = 0; t < kTiles; ++t) {
+                const float scale = half_of<true, 0>(v_params[t][m]), low = half_of<true, 1>(v_params[t][m]);
+                std::uint16_t* const to = turn + (2 * m * kRows + row0) * kCacheKeys + place0 + 4 * t;
+#pragma unroll
+                for (int i = 0; i < 4; i += 2) {
+                    const float x = prob[t][i] * scale, y = prob[t][i + 1] * scale;
+                    const std::uint32_t first = pack_pair<true>(x, y);
+                    const std::uint32_t second = pack_pair<true>(x - half_of<true, 0>(first), y - half_of<true, 1>(first));
+                    to[i * kCacheKeys] = static_cast<std::uint16_t>(first);
+                    to[(i + 1) * kCacheKeys] = static_cast<std::uint16_t>(first >> 16);
+                    to[(kRows + i) * kCacheKeys] = static_cast<std::uint16_t>(second);
+                    to[(kRows + i + 1) * kCacheKeys] = static_cast<std::uint16_t>(second >> 16);
+                    below[m][i] = __builtin_fmaf(prob[t][i], low, below[m][i]);
+                    below[m][i + 1] = __builtin_fmaf(prob[t][i + 1], low, below[m][i + 1]);
+                }
+            }
+        asm volatile("" ::: "memory");
+#pragma unroll
+        for (int m = 0; m < kGroups; ++m) {
             const uint4v v = *reinterpret_cast<const uint4v*>(block + cache_values_at(kGroups) + 64 * (16 * m + r) + 16 * g);
             const uint4v a0 = value_codes.template of<0>(v), a1 = value_codes.template of<1>(v), a2 = value_codes.template of<2>(v),
                          a3 = value_codes.template of<3>(v);
-            for (const uint4v& part_of_p : {high, low}) {
-                o[m][0] = mfma_16x16x32<true>(a0, part_of_p, o[m][0]);
-                o[m][1] = mfma_16x16x32<true>(a1, part_of_p, o[m][1]);
-                o[m][2] = mfma_16x16x32<true>(a2, part_of_p, o[m][2]);
-                o[m][3] = mfma_16x16x32<true>(a3, part_of_p, o[m][3]);
-                sixteen[m] = mfma_16x16x32<true>(ones, part_of_p, sixteen[m]);
+            // Columns: 8 rows' first parts and their second parts, or 16 rows and one part after the other.
+#pragma unroll
+            for (int part = 0; part < kTiles; ++part) {
+                const uint4v ps = *reinterpret_cast<const uint4v*>(turn + (2 * m * kRows + part * kRows + r) * kCacheKeys + 8 * g);
+                o[m][0] = mfma_16x16x32<true>(a0, ps, o[m][0]);
+                o[m][1] = mfma_16x16x32<true>(a1, ps, o[m][1]);
+                o[m][2] = mfma_16x16x32<true>(a2, ps, o[m][2]);
+                o[m][3] = mfma_16x16x32<true>(a3, ps, o[m][3]);
+                sixteen[m] = mfma_16x16x32<true>(ones, ps, sixteen[m]);
             }
         }
+        asm volatile("" ::: "memory");
     };
     // Every wave leaves when its blocks run out.
     while (steps[0] < segment.end) {
@@ -487,106 +581,123 @@ __global__ __launch_bounds__(kThreads, kGroupsPerUnit) void cache4_attention_ker
         slot = slot + 1 == kSlots ? 0 : slot + 1;
     }
     const Segment done = segment;
-    const int done_rows = rows, done_head0 = head0;
-    more = segment.end == segment.blocks && next_segment(p, segment, range_end);
-    if (more) begin_segment();
+    const int done_rows = rows;
+    std::uint16_t* const out = p.O + segment.sequence * p.o.row + head0 * p.o.head;
+    more = next_window;
+    if (more) {
+        segment = next;
+        begin_segment();
+    }
 
     // ------------------------------------------------------- merge of waves
-    row_sum = groups_sum(row_sum);
-    if (g == 0) {
-        lds_ml[wave][r][0] = row_max;
-        lds_ml[wave][r][1] = row_sum;
+    auto add = [](float x, float y) { return x + y; };
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        float4v state{row_max[i], row_reduce(row_sum[i], add), 0.0f, 0.0f};
+#pragma unroll
+        for (int m = 0; m < kGroups; ++m) state[2 + m] = row_reduce(below[m][i], add);
+        if (r == 0 && (kTiles == 2 || g < 2)) *reinterpret_cast<float4v*>(&lds_ml[wave][row0 + i][0]) = state;
     }
-    const int row = tid >> 4, f0 = 4 * (tid & 15);  // of every group
     float row_m = -INFINITY, row_l = 0.0f;
     float weight[kWaves];
-    float4v acc[kGroups];
+    float4v value[kPasses];
 #pragma unroll
-    for (int m = 0; m < kGroups; ++m) {
-        const float rest = __builtin_fmaf(-16.0f, sixteen[m][0], groups_sum(below[m]));
+    for (int x = 0; x < kPasses; ++x) {
+        const int m = x / 2;
+        const float rest = -16.0f * sixteen[m][0];
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
-            *reinterpret_cast<float4v*>(&lds_o[wave][r][16 * g + 4 * i]) =
+        for (int i = 2 * (x % 2); i < 2 * (x % 2) + 2; ++i)
+            *reinterpret_cast<float4v*>(lds_piece[wave] + (r * kQuads + 2 * g + i % 2) * 16) =
                 float4v{o[m][0][i] + rest, o[m][1][i] + rest, o[m][2][i] + rest, o[m][3][i] + rest};
         __syncthreads();
-        if (m == 0) {
+        value[x] = float4v{0.0f, 0.0f, 0.0f, 0.0f};
+        if (row < kRows) {
+            if (x == 0) {
 #pragma unroll
-            for (int w = 0; w < kWaves; ++w) row_m = fmaxf(row_m, lds_ml[w][row][0]);
+                for (int w = 0; w < kWaves; ++w) row_m = fmaxf(row_m, lds_ml[w][row][0]);
+#pragma unroll
+                for (int w = 0; w < kWaves; ++w) {
+                    // (A wave whose scores are all NaN has the maximum -inf, and a NaN sum.)
+                    const float m_w = lds_ml[w][row][0];
+                    weight[w] = m_w == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m_w - row_m);
+                    row_l += weight[w] * lds_ml[w][row][1];
+                }
+            }
 #pragma unroll
             for (int w = 0; w < kWaves; ++w) {
-                // (A wave whose scores are all NaN has the maximum -inf, and a NaN sum.)
-                const float m_w = lds_ml[w][row][0];
-                weight[w] = m_w == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m_w - row_m);
-                row_l += weight[w] * lds_ml[w][row][1];
+                float4v part = *reinterpret_cast<const float4v*>(lds_piece[w] + (row * kQuads + quad) * 16) + lds_ml[w][row][2 + m];
+                if constexpr (kTiles == 1)  // the second parts of p scale
+                    part += *reinterpret_cast<const float4v*>(lds_piece[w] + ((kRows + row) * kQuads + quad) * 16);
+                value[x] += weight[w] * part;
             }
         }
-        acc[m] = float4v{0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll
-        for (int w = 0; w < kWaves; ++w) acc[m] += weight[w] * *reinterpret_cast<const float4v*>(&lds_o[w][row][f0]);
-        __syncthreads();  // lds_o is read: the next group or segment may write it
+        __syncthreads();  // the pieces are read: the next pass or segment may write them
     }
-    const bool mine = row < done_rows;
-
-    // ------------------------------------------------------- merge of parts
-    // The ranges that have a part of this sequence and head: part i is the continued one
-    // of range first_range + i, part 0 the one to be continued.
-    bool whole = true;
     const int first_range = static_cast<int>(done.start / range_length);
     const int count = static_cast<int>((done.start + done.blocks - 1) / range_length) - first_range + 1;
-    if (count > 1) {
-        constexpr int kPartO = kTileRows * kDP, kPartMl = kTileRows * 2;
-        const Rsrc ro = shared_rows(p.part_o, std::int64_t{2} * kRanges * kPartO);
-        const Rsrc rml = shared_rows(p.part_ml, std::int64_t{2} * kRanges * kPartMl);
-        auto place_of = [&](int i) { return 2 * (first_range + i) + (i == 0 ? 1 : 0); };
-        if (mine) {
-            const int at = place_of(range - first_range);
+    if (count == 1) {
+        if (row < done_rows) store_rows(value, row_l, out);
+    } else {
+        const int place = part_place(first_range, range - first_range);
+        if (row < done_rows) {
 #pragma unroll
-            for (int x = 0; x < kGroups; ++x)
-                __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(uint4v, acc[x]), ro,
-                                                       (at * kPartO + row * kDP + 64 * x + f0) * 4, 0, kDeviceScope);
-            if (f0 == 0)
+            for (int x = 0; x < kPasses; ++x)
+                __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(uint4v, value[x]), ro, part_at(place, x), 0, kDeviceScope);
+            if (quad == 0)
                 __builtin_amdgcn_raw_buffer_store_b64(__builtin_bit_cast(uint2v, float2v{row_m, row_l}), rml,
-                                                      (at * kPartMl + 2 * row) * 4, 0, kDeviceScope);
+                                                      (place * kPartMl + 2 * row) * 4, 0, kDeviceScope);
         }
-        whole = last_arrival(p.arrivals + first_range, count, &lds_last);
-        if (whole && mine) {
-            row_m = -INFINITY;
-            row_l = 0.0f;
+        if (shares == 0)
+            shared[0] = Shared{first_range, count, done_rows, out};
+        else
+            shared[1] = Shared{first_range, count, done_rows, out};
+        ++shares;
+    }
+    }
+
+    // ------------------------------------------------------- merge of parts
+    if (shares == 0) return;
+    // As last_arrival (attention_common.h), for both parts at once.
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    __syncthreads();
+    if (lane == 0 && wave < shares) {
+        const Shared& mine = wave == 0 ? shared[0] : shared[1];
+        unsigned* const counter = p.arrivals + mine.first_range;
+        const unsigned before = __hip_atomic_fetch_add(counter, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        const bool last = before == static_cast<unsigned>(mine.count) - 1u;
+        if (last) __hip_atomic_store(counter, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        lds_last[wave] = last;
+    }
+    __syncthreads();
+#pragma unroll 1
+    for (int which = 0; which < shares; ++which) {
+        const Shared& mine = which == 0 ? shared[0] : shared[1];
+        if (!lds_last[which] || row >= mine.rows) continue;
+        float m_all = -INFINITY, l_all = 0.0f;
+        float4v sum[kPasses];
 #pragma unroll
-            for (int x = 0; x < kGroups; ++x) acc[x] = float4v{0.0f, 0.0f, 0.0f, 0.0f};
-            constexpr int kBatch = 8;
-            for (int s0 = 0; s0 < count; s0 += kBatch) {
-                float2v state[kBatch];
-                float4v value[kBatch][kGroups];
+        for (int x = 0; x < kPasses; ++x) sum[x] = float4v{0.0f, 0.0f, 0.0f, 0.0f};
+        constexpr int kBatch = 4;
+        for (int s0 = 0; s0 < mine.count; s0 += kBatch) {
+            float2v state[kBatch];
+            float4v part[kBatch][kPasses];
 #pragma unroll
-                for (int u = 0; u < kBatch; ++u) {
-                    const int at = place_of(min(s0 + u, count - 1));
-                    state[u] = __builtin_bit_cast(
-                        float2v, __builtin_amdgcn_raw_buffer_load_b64(rml, (at * kPartMl + 2 * row) * 4, 0, kDeviceScope));
+            for (int u = 0; u < kBatch; ++u) {
+                const int place = part_place(mine.first_range, min(s0 + u, mine.count - 1));
+                state[u] = __builtin_bit_cast(
+                    float2v, __builtin_amdgcn_raw_buffer_load_b64(rml, (place * kPartMl + 2 * row) * 4, 0, kDeviceScope));
 #pragma unroll
-                    for (int x = 0; x < kGroups; ++x)
-                        value[u][x] = __builtin_bit_cast(
-                            float4v, __builtin_amdgcn_raw_buffer_load_b128(ro, (at * kPartO + row * kDP + 64 * x + f0) * 4, 0,
-                                                                           kDeviceScope));
-                }
-                merge_batch<kBatch, true>(
-                    row_m, row_l, count - s0, [&](int u) __attribute__((always_inline)) { return state[u]; },
-                    [&](int u, PartWeights w) __attribute__((always_inline)) {
-#pragma unroll
-                        for (int x = 0; x < kGroups; ++x) acc[x] = merged(acc[x], value[u][x], w);
-                    });
+                for (int x = 0; x < kPasses; ++x)
+                    part[u][x] = __builtin_bit_cast(float4v, __builtin_amdgcn_raw_buffer_load_b128(ro, part_at(place, x), 0, kDeviceScope));
             }
-        }
-    }
-    if (whole && mine) {
-        const float inverse = row_l == 0.0f ? 0.0f : 1.0f / row_l;  // 0: no token
-        std::uint16_t* const out = p.O + done.sequence * p.o.row + (done_head0 + row) * p.o.head + f0;
+            merge_batch<kBatch, true>(
+                m_all, l_all, mine.count - s0, [&](int u) __attribute__((always_inline)) { return state[u]; },
+                [&](int u, PartWeights w) __attribute__((always_inline)) {
 #pragma unroll
-        for (int x = 0; x < kGroups; ++x)
-            if (64 * x + f0 < d)
-                *reinterpret_cast<uint2v*>(out + 64 * x) = uint2v{pack_pair<kBf16>(acc[x][0] * inverse, acc[x][1] * inverse),
-                                                                 pack_pair<kBf16>(acc[x][2] * inverse, acc[x][3] * inverse)};
-    }
+                    for (int x = 0; x < kPasses; ++x) sum[x] = merged(sum[x], part[u][x], w);
+                });
+        }
+        store_rows(sum, l_all, mine.out);
     }
 }
 
@@ -631,17 +742,27 @@ extern "C" int tilemix_attention_cache4(const TileMixCache4AttentionArgs* args, 
     // Ranges of at least kLeastSteps blocks.
     const std::int64_t items = static_cast<std::int64_t>(a.batch) * a.kv_heads * p.tiles;
     const std::int64_t most = (p.most_tokens - 1) / kCacheKeys + 1;  // blocks of one of them
-    p.ranges = static_cast<int>(std::min<std::int64_t>(kRanges, items > kRanges * kLeastSteps ? kRanges : (items * most - 1) / kLeastSteps + 1));
+    const int ranges = p.group <= 8 ? kRanges : kRanges16;
+    p.ranges = static_cast<int>(std::min<std::int64_t>(ranges, items > ranges * kLeastSteps ? ranges : (items * most - 1) / kLeastSteps + 1));
     const hipError_t found = check_device();
     if (found != hipSuccess) return found;
     const hipStream_t s = static_cast<hipStream_t>(stream);
     const bool bf16 = a.dtype == TILEMIX_DTYPE_BF16;
     const unsigned workgroups = static_cast<unsigned>(p.ranges);
-    if (p.cache.groups == 1)
-        bf16 ? cache4_attention_kernel<1, true><<<workgroups, kThreads, 0, s>>>(p)
-             : cache4_attention_kernel<1, false><<<workgroups, kThreads, 0, s>>>(p);
+    auto launch = [&](auto groups, auto rows) {
+        constexpr int kGroups = decltype(groups)::value, kRows = decltype(rows)::value;
+        if (bf16)
+            cache4_attention_kernel<kGroups, true, kRows><<<workgroups, kThreads, 0, s>>>(p);
+        else
+            cache4_attention_kernel<kGroups, false, kRows><<<workgroups, kThreads, 0, s>>>(p);
+    };
+    using One = std::integral_constant<int, 1>;
+    using Two = std::integral_constant<int, 2>;
+    using Eight = std::integral_constant<int, 8>;
+    using Sixteen = std::integral_constant<int, 16>;
+    if (p.group <= 8)
+        p.cache.groups == 1 ? launch(One{}, Eight{}) : launch(Two{}, Eight{});
     else
-        bf16 ? cache4_attention_kernel<2, true><<<workgroups, kThreads, 0, s>>>(p)
-             : cache4_attention_kernel<2, false><<<workgroups, kThreads, 0, s>>>(p);
+        p.cache.groups == 1 ? launch(One{}, Sixteen{}) : launch(Two{}, Sixteen{});
     return hipGetLastError();
 }
