@@ -39,12 +39,12 @@ namespace {
 
 constexpr int kWaves = 4;
 constexpr int kThreads = kWaves * kWave;
-constexpr int kGroupsPerUnit = 3;  // workgroups of a CU that registers are allocated for
+constexpr int kGroupsPerUnit = 2;  // workgroups of a CU that registers are allocated for
 constexpr int kSlots = 2;         // blocks in a wave's ring: one computed, the others under way
 constexpr int kTileRows = 16;     // query rows of a workgroup
-constexpr int kLeastSteps = 8;  // blocks of a range: two for each wave
-constexpr int kRanges16 = 512;  // the same of the kernel with 16 rows, which takes more LDS
-constexpr int kRanges = 768;    // at most: workgroups that the device holds at once
+constexpr int kLeastSteps = 16;  // places of a range at least
+constexpr int kSwitch = 8;       // places of a range that the step to another sequence counts for
+constexpr int kRanges = 512;    // at most: workgroups that the device holds at once
 // The workspace: arrival counters, then rows of O and their states for the two parts
 // (one continued, one to be continued) that a range can have.
 constexpr std::size_t kWorkspaceBytes =
@@ -151,66 +151,78 @@ __device__ __forceinline__ unsigned lane_value(unsigned v, int lane) {
 }
 
 __device__ __forceinline__ int length_of(const DecodeParams& p, int b) { return min(max(p.lengths[b], 0), p.most_tokens); }
-// Blocks of sequence b: under 2^26, so that 64 sequences' fit 32 bits. An empty one counts
-// as one block (without a page), so that some range has it and writes its zeros.
-__device__ __forceinline__ unsigned blocks_of(const DecodeParams& p, int b) {
-    return b < p.batch ? static_cast<unsigned>(max((length_of(p, b) + kCacheKeys - 1) / kCacheKeys, 1)) : 0u;
-}
+// Blocks of sequence b. An empty one counts as one block (without a page), so that some
+// range has it and writes its zeros.
+__device__ __forceinline__ int blocks_of(int length) { return max((length + kCacheKeys - 1) / kCacheKeys, 1); }
 
-// Blocks first .. end - 1 of a sequence and head (of its `blocks`).
+// Positions: the sequences of head 0, then of head 1, ... (a head: one key head's row
+// tile), each with its blocks and `gap` places more, which stand for the time that a
+// workgroup takes from one sequence to the next. With a sequence's heads side by side, a
+// short one's would all fall to the same workgroup (64 sequences of 1 to 16384 tokens, 8
+// heads: 121 us so, 93 as it is). All positions fit 30 bits (checked by the host).
 struct Segment {
-    int sequence, item;  // item: head * tiles + row tile
-    int first, end, blocks;
-    int length;               // tokens of the sequence
-    std::int64_t start;       // the sequence and head's first block, among all
+    int sequence, head;
+    int first, end, blocks;  // blocks first .. end - 1 of the sequence's
+    int length;              // tokens of the sequence
+    int start;               // position of its first block
 };
 
-// The length of a range, and the segment in which range number `range` begins; false past
-// the last range. Wave-uniform.
-__device__ __forceinline__ bool first_segment(const DecodeParams& p, int range, int lane, Segment& segment, std::int64_t& length) {
-    const int heads = p.cache.kv_heads * p.tiles;
-    const unsigned kept = blocks_of(p, lane);  // of the first kWave sequences
-    std::int64_t total = lane_value(prefix_sum(kept), kWave - 1);
-    for (int base = kWave; base < p.batch; base += kWave) total += lane_value(prefix_sum(blocks_of(p, base + lane)), kWave - 1);
-    total *= heads;
-    length = max((total + p.ranges - 1) / p.ranges, std::int64_t{kLeastSteps});
-    const std::int64_t begin = range * length;
+struct Plan {
+    int length;  // of a range
+    int gap;
+};
+
+// The ranges, and the segment in which range number `range` begins; false where it has
+// none. Wave-uniform.
+__device__ __forceinline__ bool first_segment(const DecodeParams& p, int range, int lane, Segment& segment, Plan& plan) {
+    const unsigned heads = p.cache.kv_heads * p.tiles;
+    auto blocks_at = [&](int b) __attribute__((always_inline)) { return b < p.batch ? blocks_of(length_of(p, b)) : 0; };
+    const int kept = blocks_at(lane);  // of the first kWave sequences
+    const int sequence0 = __builtin_amdgcn_readfirstlane(kept);
+    bool alike = __all(kept == sequence0 || lane >= p.batch);
+    unsigned blocks = lane_value(prefix_sum(kept), kWave - 1);  // of a head
+    for (int base = kWave; base < p.batch; base += kWave) {
+        const int mine = blocks_at(base + lane);
+        alike = alike && __all(mine == sequence0 || base + lane >= p.batch);
+        blocks += lane_value(prefix_sum(mine), kWave - 1);
+    }
+    plan.gap = kSwitch;
+    unsigned one = blocks + p.batch * kSwitch, total = one * heads;
+    plan.length = max(static_cast<int>((total + p.ranges - 1) / p.ranges), kLeastSteps);
+    const unsigned items = p.batch * heads;
+    if (alike && items <= static_cast<unsigned>(p.ranges)) {
+        // Each sequence and head in as many whole ranges as there are for it, if that is
+        // hardly more for each: no range then has parts of two, which takes it longer (2
+        // sequences of 32768 tokens, 16 heads: 40.7 us, 35.4 so).
+        const unsigned each = p.ranges / items;
+        const int length = max(static_cast<int>((sequence0 + each - 1) / each), kLeastSteps);
+        if (length <= plan.length + kSwitch) {
+            plan.gap = (length - sequence0 % length) % length;
+            plan.length = length;
+            one = blocks + p.batch * plan.gap;
+            total = one * heads;
+        }
+    }
+    const unsigned begin = static_cast<unsigned>(range) * plan.length;
     if (begin >= total) return false;
-    std::int64_t before = 0;  // blocks of one head in the sequences before
+    segment.head = static_cast<int>(begin / one);
+    const unsigned inside = begin - segment.head * one;
+    unsigned before = 0;
     for (int base = 0;; base += kWave) {
-        const unsigned mine = base == 0 ? kept : blocks_of(p, base + lane);
-        const unsigned sum = prefix_sum(mine);
-        const std::uint64_t past = __ballot((before + sum) * heads > begin);
+        const unsigned mine = base == 0 ? kept : blocks_at(base + lane);
+        const unsigned sum = prefix_sum(base + lane < p.batch ? mine + plan.gap : 0u) + before;
+        const std::uint64_t past = __ballot(sum > inside);
         if (past) {
             const int at = __builtin_ctzll(past);
             segment.sequence = base + at;
             segment.blocks = static_cast<int>(lane_value(mine, at));
-            const std::int64_t sequence_start = (before + lane_value(sum, at) - segment.blocks) * heads;
-            segment.item = static_cast<int>((begin - sequence_start) / segment.blocks);
-            segment.start = sequence_start + static_cast<std::int64_t>(segment.item) * segment.blocks;
-            segment.first = static_cast<int>(begin - segment.start);
+            segment.start = static_cast<int>(segment.head * one + lane_value(sum, at)) - segment.blocks - plan.gap;
+            segment.first = static_cast<int>(begin) - segment.start;
             break;
         }
-        before += lane_value(sum, kWave - 1);
+        before = lane_value(sum, kWave - 1);
     }
-    segment.length = length_of(p, segment.sequence);
-    segment.end = static_cast<int>(min(static_cast<std::int64_t>(segment.blocks), segment.first + length));
-    return true;
-}
-
-// The segment after one that ends its sequence and head before block `end` of all; false
-// where there is none.
-__device__ __forceinline__ bool next_segment(const DecodeParams& p, Segment& s, std::int64_t end) {
-    s.start += s.blocks;
-    if (s.start >= end) return false;
-    s.first = 0;
-    if (++s.item == p.cache.kv_heads * p.tiles) {
-        s.item = 0;
-        if (++s.sequence >= p.batch) return false;
-        s.length = length_of(p, s.sequence);
-        s.blocks = max((s.length + kCacheKeys - 1) / kCacheKeys, 1);
-    }
-    s.end = static_cast<int>(min(static_cast<std::int64_t>(s.blocks), end - s.start));
+    segment.end = min(segment.blocks, segment.first + plan.length);
     return true;
 }
 
@@ -234,9 +246,9 @@ __global__ __launch_bounds__(kThreads, kGroupsPerUnit) void cache4_attention_ker
     constexpr int kLoads = 3 * kGroups;  // of a block: 2 kGroups KiB of codes, then 256-byte pieces of parameters
     __shared__ __attribute__((aligned(16))) unsigned char lds_blocks[kWaves][kSlots][kBlockBytes];  // a ring per wave
     // A wave's piece: p scale on its way to the matrix operand's layout while blocks are computed,
-    // 32 features of O at a segment's end.
-    constexpr int kTurnBytes = kGroups * 2 * kRows * kCacheKeys * 2, kQuads = 8;
-    constexpr int kPieceBytes = kTurnBytes > kTileRows * kQuads * 16 ? kTurnBytes : kTileRows * kQuads * 16;
+    // O at a segment's end.
+    constexpr int kPieceBytes = kRows * kDP * 4;
+    static_assert(kPieceBytes >= kGroups * 2 * kRows * kCacheKeys * 2, "p scale fits");
     __shared__ __attribute__((aligned(16))) unsigned char lds_piece[kWaves][kPieceBytes];
     __shared__ __attribute__((aligned(16))) float lds_ml[kWaves][kTileRows][4];  // maximum, sum, sum p minimum of both groups
     __shared__ int lds_last[2];
@@ -259,32 +271,73 @@ __global__ __launch_bounds__(kThreads, kGroupsPerUnit) void cache4_attention_ker
         return x;
     };
     Segment segment;
-    std::int64_t range_length;
+    Plan plan;
     const int range = blockIdx.x;
-    if (!first_segment(p, range, lane, segment, range_length)) return;
-    const std::int64_t range_end = (range + std::int64_t{1}) * range_length;
+    if (!first_segment(p, range, lane, segment, plan)) return;
+    const int range_end = (range + 1) * plan.length;
     const int d = p.d;
     const int per_page = p.cache.page_size / kCacheKeys;
 
-    // -------------------------------------------------- blocks of a segment
-    // A wave takes blocks first + wave, + kWaves, ... of a segment. Lane l of the window
-    // holds the page of number window + l of the sequence.
-    int step, page, inside, window, window_page;
+    // Lengths of sequences lengths_at .. + 63, one a lane.
+    int lengths_at = segment.sequence;
+    int lengths = lengths_at + lane < p.batch ? length_of(p, lengths_at + lane) : 0;
+    segment.length = __builtin_amdgcn_readfirstlane(lengths);
+    // The segment after `s` in this range.
+    auto after = [&](const Segment& s, Segment& out) __attribute__((always_inline)) {
+        out = s;
+        out.start += s.blocks + plan.gap;
+        if (s.end < s.blocks || out.start >= range_end) return false;
+        out.first = 0;
+        if (++out.sequence == p.batch) {
+            out.sequence = 0;
+            if (++out.head == p.cache.kv_heads * p.tiles) return false;
+        }
+        if (static_cast<unsigned>(out.sequence - lengths_at) >= kWave) {
+            lengths_at = out.sequence;
+            lengths = lengths_at + lane < p.batch ? length_of(p, lengths_at + lane) : 0;
+        }
+        out.length = __builtin_amdgcn_readlane(lengths, out.sequence - lengths_at);
+        out.blocks = blocks_of(out.length);
+        out.end = min(out.blocks, range_end - out.start);
+        return true;
+    };
+    // A range that begins in the places after a sequence's blocks begins with the next one.
+    if (segment.first >= segment.blocks) {
+        segment.end = segment.blocks;
+        const Segment before = segment;
+        if (!after(before, segment)) return;
+    }
+    auto head_of = [&](const Segment& s) __attribute__((always_inline)) { return p.tiles == 1 ? s.head : s.head / p.tiles; };
+
+    // ------------------------------------------------- a wave's blocks, in turn
+    // Blocks first + wave, + kWaves, ... of a segment, then of the next: a segment's first
+    // blocks are under way before the one before is done. Lane l of the window holds
+    // page number window + l of the sequence.
+    int step, end, page, inside, pages, window, window_page;
     const std::int32_t* table;
     const std::uint8_t* head_data;
+    const std::uint8_t* data = nullptr;
+    int bytes = 0;  // of the block at data; 0: none, and its loads touch no memory
     auto load_window = [&]() __attribute__((always_inline)) {
         window = page;
-        const int pages = (segment.length + p.cache.page_size - 1) / p.cache.page_size;
         window_page = window + lane < pages ? table[window + lane] : -1;
         // Waited for here, once in 64 pages: read in the loop as a load that may be under way,
         // it would make every block wait for all of the blocks' loads.
         wait_vmcnt<0>();
     };
-    const std::uint8_t* data = nullptr;
-    int bytes = 0;  // of the block at data: 0 past the segment's last, whose loads then touch no memory
+    auto enter = [&](const Segment& s) __attribute__((always_inline)) {
+        table = p.table + s.sequence * p.table_stride;
+        head_data = p.cache.data + head_of(s) * p.cache.head_bytes;
+        pages = (s.length + p.cache.page_size - 1) / p.cache.page_size;
+        end = s.end;
+        step = s.first + wave;
+        page = step / per_page;
+        inside = step - page * per_page;
+    };
     // From `step` on, the first block whose page is one of the cache.
     auto find = [&]() __attribute__((always_inline)) {
-        while (step < segment.end) {
+        bytes = 0;
+        while (step < end) {
             if (page - window >= kWave) load_window();
             const int number = __builtin_amdgcn_readlane(window_page, page - window);
             if (number >= 0 && number < p.cache.pages) {
@@ -296,13 +349,6 @@ __global__ __launch_bounds__(kThreads, kGroupsPerUnit) void cache4_attention_ker
             inside += kWaves;
             while (inside >= per_page) inside -= per_page, ++page;
         }
-        bytes = 0;
-    };
-    auto next_block = [&]() __attribute__((always_inline)) {
-        step += kWaves;
-        inside += kWaves;
-        while (inside >= per_page) inside -= per_page, ++page;
-        find();
     };
     // The block at data into a slot of the wave's ring; past the segment's end zeros, so
     // that the number of loads under way is always known.
@@ -317,56 +363,55 @@ __global__ __launch_bounds__(kThreads, kGroupsPerUnit) void cache4_attention_ker
             load_dwords_to_lds(rs, to + cache_key_params_at(kGroups) + 256 * x, cache_key_params_at(kGroups) + 256 * x + 4 * lane);
     };
 
-    // ------------------------------------------------------------ a segment
-    int steps[kSlots];  // of the blocks in the ring, the one to be computed first
-    int slot = 0;       // its place
-    uint4v qf[kGroups][2];
-    int rows = 0, head0 = 0;
-    Segment next;
-    bool more = true, next_window = false;
-    int next_page = 0;  // window of the wave's first pages of `next`
-    auto look_ahead = [&]() __attribute__((always_inline)) {
-        next = segment;
-        next_window = segment.end == segment.blocks && next_segment(p, next, range_end);
-        if (next_window) {
-            const int pages = (next.length + p.cache.page_size - 1) / p.cache.page_size, first = wave / per_page;
-            next_page = first + lane < pages ? p.table[next.sequence * p.table_stride + first + lane] : -1;
-        }
-    };
-    // Queries and the wave's first blocks of `segment`, on their way.
-    auto begin_segment = [&]() __attribute__((always_inline)) {
-        const int head = segment.item / p.tiles, tile = segment.item - head * p.tiles;
-        rows = min(p.group - tile * kTileRows, kTileRows);
-        head0 = head * p.group + tile * kTileRows;
-        table = p.table + segment.sequence * p.table_stride;
-        head_data = p.cache.data + head * p.cache.head_bytes;
-        step = segment.first + wave;
-        page = step / per_page;
-        inside = step - page * per_page;
-        if (next_window) {
-            window = page;
-            window_page = next_page;
-        } else {
-            load_window();
-        }
+    // Queries of a segment: row r (mod kRows) of its tile.
+    auto load_queries = [&](uint4v (&to)[kGroups][2], const Segment& s) __attribute__((always_inline)) {
+        const int head = head_of(s), tile = s.head - head * p.tiles;
+        const int query = tile * kTileRows + r % kRows;
+        const std::uint16_t* const from = p.Q + s.sequence * p.q.row + (head * p.group + query) * p.q.head;
 #pragma unroll
         for (int m = 0; m < kGroups; ++m)
 #pragma unroll
             for (int w = 0; w < 2; ++w) {
                 const int feature = 64 * m + 16 * g + 8 * w;
-                qf[m][w] = uint4v{0u, 0u, 0u, 0u};
-                if (r % kRows < rows && feature < d)
-                    qf[m][w] = *reinterpret_cast<const uint4v*>(p.Q + segment.sequence * p.q.row + (head0 + r % kRows) * p.q.head + feature);
+                to[m][w] = query < p.group && feature < d ? *reinterpret_cast<const uint4v*>(from + feature) : uint4v{0u, 0u, 0u, 0u};
             }
-        find();
-        slot = 0;
-        __builtin_amdgcn_s_waitcnt(0xc07f);  // lgkmcnt(0): the ring is read
-#pragma unroll
-        for (int x = 0; x < kSlots - 1; ++x) {
-            if (x > 0) next_block();
-            steps[x] = step;
-            issue(x);
+    };
+    // What follows `segment`: its queries and the window of the wave's first pages are loaded
+    // while `segment` is computed.
+    Segment next;
+    bool has_next, in_next = false;  // in_next: the wave's blocks have got to `next`
+    int next_page = 0;
+    uint4v qf[kGroups][2], next_qf[kGroups][2];
+    auto look_ahead = [&]() __attribute__((always_inline)) {
+        has_next = after(segment, next);
+        if (has_next) {
+            const int count = (next.length + p.cache.page_size - 1) / p.cache.page_size, first = wave / per_page;
+            next_page = first + lane < count ? p.table[next.sequence * p.table_stride + first + lane] : -1;
+            load_queries(next_qf, next);
         }
+    };
+    // The ring: what each slot holds, the one to be computed first. Steps of `segment`,
+    // kInNext more for those of `next`, kNone.
+    constexpr int kInNext = 1 << 28, kNone = -1;
+    int held[kSlots];
+    int slot = 0;  // place of held[0]
+    auto take_next = [&](int to) __attribute__((always_inline)) {
+        if (bytes == 0 && !in_next && has_next) {
+            enter(next);
+            window = page;
+            window_page = next_page;
+            in_next = true;
+            find();
+        }
+        issue(to);
+        const int what = bytes == 0 ? kNone : step + (in_next ? kInNext : 0);
+        if (bytes != 0) {
+            step += kWaves;
+            inside += kWaves;
+            while (inside >= per_page) inside -= per_page, ++page;
+            find();
+        }
+        return what;
     };
     const Codes<kBf16> key_codes;
     const Codes<true> value_codes;
@@ -374,15 +419,20 @@ __global__ __launch_bounds__(kThreads, kGroupsPerUnit) void cache4_attention_ker
     // What the range has a part of, at most two: merged, where this workgroup is the last
     // to arrive, at the end.
     struct Shared {
-        int first_range, count, rows;
+        Segment segment;
         std::uint16_t* out;
     };
     Shared shared[2];
     int shares = 0;
-    const int row = tid / kQuads, quad = tid % kQuads;  // a thread's row and 4 features in a pass of the merges
-    constexpr int kPasses = 2 * kGroups;
-    const int thread_feature = 16 * (quad >> 1) + 4 * (quad & 1);  // + 32 (pass / 2) * 2 + 8 (pass % 2)
-    auto feature_of = [&](int pass) __attribute__((always_inline)) { return 64 * (pass / 2) + 8 * (pass % 2) + thread_feature; };
+    // A thread's row and 4 kPasses features in the merges
+    // (with 8 rows of 64 features half of the threads have none).
+    constexpr int kThreadsPerRow = kThreads / kRows < kDP / 4 ? kThreads / kRows : kDP / 4, kPasses = kDP / 4 / kThreadsPerRow;
+    const bool has_row = tid / kThreadsPerRow < kRows;
+    const int row = has_row ? tid / kThreadsPerRow : 0, f0 = 4 * (tid % kThreadsPerRow);
+    auto feature_of = [&](int pass) __attribute__((always_inline)) { return f0 + 4 * kThreadsPerRow * pass; };
+    auto rows_of = [&](const Segment& s) __attribute__((always_inline)) {
+        return min(p.group - (s.head - head_of(s) * p.tiles) * kTileRows, kRows);
+    };
     auto store_rows = [&](const float4v (&value)[kPasses], float l, std::uint16_t* out) __attribute__((always_inline)) {
         const float inverse = l == 0.0f ? 0.0f : 1.0f / l;  // 0: no token
 #pragma unroll
@@ -398,12 +448,16 @@ __global__ __launch_bounds__(kThreads, kGroupsPerUnit) void cache4_attention_ker
     const Rsrc ro = shared_rows(p.part_o, std::int64_t{2} * kRanges * kPartO);
     const Rsrc rml = shared_rows(p.part_ml, std::int64_t{2} * kRanges * kPartMl);
     auto part_place = [](int first_range, int i) { return 2 * (first_range + i) + (i == 0 ? 1 : 0); };
-    auto part_at = [&](int place, int pass) __attribute__((always_inline)) {
-        return (place * kPartO + (pass * kTileRows + row) * (4 * kQuads) + 4 * quad) * 4;
-    };
-    begin_segment();
-    while (more) {
+    auto part_at = [&](int place, int pass) __attribute__((always_inline)) { return (place * kPartO + row * kDP + feature_of(pass)) * 4; };
+
+    enter(segment);
+    load_window();
+    load_queries(qf, segment);
     look_ahead();
+    find();
+#pragma unroll
+    for (int x = 0; x < kSlots - 1; ++x) held[x] = take_next(x);
+    for (;;) {
     // q_sum[m][i]: of the features of row row0 + i.
     float4v q_sum[kGroups];
 #pragma unroll
@@ -566,27 +620,23 @@ __global__ __launch_bounds__(kThreads, kGroupsPerUnit) void cache4_attention_ker
         }
         asm volatile("" ::: "memory");
     };
-    // Every wave leaves when its blocks run out.
-    while (steps[0] < segment.end) {
-        next_block();
-        steps[kSlots - 1] = step;
-        // The slot that the block before was read from: those reads are done.
+    // Until the wave's blocks of the segment run out. (One that had none left for the ring
+    // passes a place by as soon as there is a next segment to fill it from.)
+    for (;;) {
+        const int now = held[0];
+        const bool mine = now >= 0 && now < kInNext;
+        if (!mine && !(now == kNone && has_next && !in_next)) break;
+        // Into the slot that the block before was read from: those reads are done.
         __builtin_amdgcn_s_waitcnt(0xc07f);  // lgkmcnt(0)
-        issue(slot == 0 ? kSlots - 1 : slot - 1);
-        wait_vmcnt<(kSlots - 1) * kLoads>();  // all but the kSlots - 1 blocks after this one
-        asm volatile("" ::: "memory");
-        compute(steps[0]);
+        held[kSlots - 1] = take_next(slot == 0 ? kSlots - 1 : slot - 1);
+        if (mine) {
+            wait_vmcnt<(kSlots - 1) * kLoads>();  // all but the kSlots - 1 blocks after this one
+            asm volatile("" ::: "memory");
+            compute(now);
+        }
 #pragma unroll
-        for (int x = 0; x + 1 < kSlots; ++x) steps[x] = steps[x + 1];
+        for (int x = 0; x + 1 < kSlots; ++x) held[x] = held[x + 1];
         slot = slot + 1 == kSlots ? 0 : slot + 1;
-    }
-    const Segment done = segment;
-    const int done_rows = rows;
-    std::uint16_t* const out = p.O + segment.sequence * p.o.row + head0 * p.o.head;
-    more = next_window;
-    if (more) {
-        segment = next;
-        begin_segment();
     }
 
     // ------------------------------------------------------- merge of waves
@@ -598,92 +648,114 @@ __global__ __launch_bounds__(kThreads, kGroupsPerUnit) void cache4_attention_ker
         for (int m = 0; m < kGroups; ++m) state[2 + m] = row_reduce(below[m][i], add);
         if (r == 0 && (kTiles == 2 || g < 2)) *reinterpret_cast<float4v*>(&lds_ml[wave][row0 + i][0]) = state;
     }
-    float row_m = -INFINITY, row_l = 0.0f;
-    float weight[kWaves];
-    float4v value[kPasses];
 #pragma unroll
-    for (int x = 0; x < kPasses; ++x) {
-        const int m = x / 2;
+    for (int m = 0; m < kGroups; ++m) {
         const float rest = -16.0f * sixteen[m][0];
 #pragma unroll
-        for (int i = 2 * (x % 2); i < 2 * (x % 2) + 2; ++i)
-            *reinterpret_cast<float4v*>(lds_piece[wave] + (r * kQuads + 2 * g + i % 2) * 16) =
-                float4v{o[m][0][i] + rest, o[m][1][i] + rest, o[m][2][i] + rest, o[m][3][i] + rest};
-        __syncthreads();
-        value[x] = float4v{0.0f, 0.0f, 0.0f, 0.0f};
-        if (row < kRows) {
-            if (x == 0) {
+        for (int i = 0; i < 4; ++i) {
+            float4v quad{o[m][0][i] + rest, o[m][1][i] + rest, o[m][2][i] + rest, o[m][3][i] + rest};
+            if constexpr (kTiles == 1) {  // the second parts of p scale, 8 columns on
 #pragma unroll
-                for (int w = 0; w < kWaves; ++w) row_m = fmaxf(row_m, lds_ml[w][row][0]);
-#pragma unroll
-                for (int w = 0; w < kWaves; ++w) {
-                    // (A wave whose scores are all NaN has the maximum -inf, and a NaN sum.)
-                    const float m_w = lds_ml[w][row][0];
-                    weight[w] = m_w == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m_w - row_m);
-                    row_l += weight[w] * lds_ml[w][row][1];
+                for (int f = 0; f < 4; ++f) {
+                    const float x = quad[f];
+                    quad[f] = x + __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, x), 0x128, 0xf, 0xf, false));
                 }
             }
-#pragma unroll
-            for (int w = 0; w < kWaves; ++w) {
-                float4v part = *reinterpret_cast<const float4v*>(lds_piece[w] + (row * kQuads + quad) * 16) + lds_ml[w][row][2 + m];
-                if constexpr (kTiles == 1)  // the second parts of p scale
-                    part += *reinterpret_cast<const float4v*>(lds_piece[w] + ((kRows + row) * kQuads + quad) * 16);
-                value[x] += weight[w] * part;
-            }
+            if (r < kRows) *reinterpret_cast<float4v*>(lds_piece[wave] + (r * kDP + 64 * m + 16 * g + 4 * i) * 4) = quad;
         }
-        __syncthreads();  // the pieces are read: the next pass or segment may write them
     }
-    const int first_range = static_cast<int>(done.start / range_length);
-    const int count = static_cast<int>((done.start + done.blocks - 1) / range_length) - first_range + 1;
-    if (count == 1) {
-        if (row < done_rows) store_rows(value, row_l, out);
+    __syncthreads();
+    float row_m = -INFINITY, row_l = 0.0f;
+    float4v value[kPasses];
+#pragma unroll
+    for (int x = 0; x < kPasses; ++x) value[x] = float4v{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+    for (int w = 0; w < kWaves; ++w) row_m = fmaxf(row_m, lds_ml[w][row][0]);
+#pragma unroll
+    for (int w = 0; w < kWaves; ++w) {
+        // (A wave whose scores are all NaN has the maximum -inf, and a NaN sum.)
+        const float m_w = lds_ml[w][row][0];
+        const float weight = m_w == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m_w - row_m);
+        row_l += weight * lds_ml[w][row][1];
+#pragma unroll
+        for (int x = 0; x < kPasses; ++x)
+            value[x] += weight * (*reinterpret_cast<const float4v*>(lds_piece[w] + (row * kDP + feature_of(x)) * 4) +
+                                  lds_ml[w][row][2 + feature_of(x) / kCacheGroup]);
+    }
+    const bool live = has_row && row < rows_of(segment);
+    std::uint16_t* out;
+    {
+        const int head = head_of(segment), tile = segment.head - head * p.tiles;
+        out = p.O + segment.sequence * p.o.row + (head * p.group + tile * kTileRows) * p.o.head;
+    }
+    if (segment.first == 0 && segment.end == segment.blocks) {
+        if (live) store_rows(value, row_l, out);
     } else {
-        const int place = part_place(first_range, range - first_range);
-        if (row < done_rows) {
+        const int place = 2 * range + (segment.first == 0 ? 1 : 0);
+        if (live) {
 #pragma unroll
             for (int x = 0; x < kPasses; ++x)
                 __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(uint4v, value[x]), ro, part_at(place, x), 0, kDeviceScope);
-            if (quad == 0)
+            if (f0 == 0)
                 __builtin_amdgcn_raw_buffer_store_b64(__builtin_bit_cast(uint2v, float2v{row_m, row_l}), rml,
                                                       (place * kPartMl + 2 * row) * 4, 0, kDeviceScope);
         }
         if (shares == 0)
-            shared[0] = Shared{first_range, count, done_rows, out};
+            shared[0] = Shared{segment, out};
         else
-            shared[1] = Shared{first_range, count, done_rows, out};
+            shared[1] = Shared{segment, out};
         ++shares;
     }
+    if (!has_next) break;
+    __syncthreads();  // the pieces are read: the next segment writes them
+    segment = next;
+    in_next = false;
+#pragma unroll
+    for (int x = 0; x < kSlots - 1; ++x)
+        if (held[x] != kNone) held[x] -= kInNext;
+#pragma unroll
+    for (int m = 0; m < kGroups; ++m)
+#pragma unroll
+        for (int w = 0; w < 2; ++w) qf[m][w] = next_qf[m][w];
+    look_ahead();
     }
 
     // ------------------------------------------------------- merge of parts
     if (shares == 0) return;
     // As last_arrival (attention_common.h), for both parts at once.
+    auto first_range_of = [&](const Segment& s) __attribute__((always_inline)) {
+        return s.first == 0 ? range : s.start / plan.length;
+    };
+    auto count_of = [&](const Segment& s) __attribute__((always_inline)) {
+        return (s.start + s.blocks - 1) / plan.length - first_range_of(s) + 1;
+    };
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
     __syncthreads();
     if (lane == 0 && wave < shares) {
-        const Shared& mine = wave == 0 ? shared[0] : shared[1];
-        unsigned* const counter = p.arrivals + mine.first_range;
+        const Segment mine = wave == 0 ? shared[0].segment : shared[1].segment;
+        unsigned* const counter = p.arrivals + first_range_of(mine);
         const unsigned before = __hip_atomic_fetch_add(counter, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-        const bool last = before == static_cast<unsigned>(mine.count) - 1u;
+        const bool last = before == static_cast<unsigned>(count_of(mine)) - 1u;
         if (last) __hip_atomic_store(counter, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
         lds_last[wave] = last;
     }
     __syncthreads();
 #pragma unroll 1
     for (int which = 0; which < shares; ++which) {
-        const Shared& mine = which == 0 ? shared[0] : shared[1];
-        if (!lds_last[which] || row >= mine.rows) continue;
+        const Shared mine = which == 0 ? shared[0] : shared[1];
+        if (!lds_last[which] || !has_row || row >= rows_of(mine.segment)) continue;
+        const int first_range = first_range_of(mine.segment), count = count_of(mine.segment);
         float m_all = -INFINITY, l_all = 0.0f;
         float4v sum[kPasses];
 #pragma unroll
         for (int x = 0; x < kPasses; ++x) sum[x] = float4v{0.0f, 0.0f, 0.0f, 0.0f};
-        constexpr int kBatch = 4;
-        for (int s0 = 0; s0 < mine.count; s0 += kBatch) {
+        constexpr int kBatch = 16 / kPasses;
+        for (int s0 = 0; s0 < count; s0 += kBatch) {
             float2v state[kBatch];
             float4v part[kBatch][kPasses];
 #pragma unroll
             for (int u = 0; u < kBatch; ++u) {
-                const int place = part_place(mine.first_range, min(s0 + u, mine.count - 1));
+                const int place = part_place(first_range, min(s0 + u, count - 1));
                 state[u] = __builtin_bit_cast(
                     float2v, __builtin_amdgcn_raw_buffer_load_b64(rml, (place * kPartMl + 2 * row) * 4, 0, kDeviceScope));
 #pragma unroll
@@ -691,7 +763,7 @@ __global__ __launch_bounds__(kThreads, kGroupsPerUnit) void cache4_attention_ker
                     part[u][x] = __builtin_bit_cast(float4v, __builtin_amdgcn_raw_buffer_load_b128(ro, part_at(place, x), 0, kDeviceScope));
             }
             merge_batch<kBatch, true>(
-                m_all, l_all, mine.count - s0, [&](int u) __attribute__((always_inline)) { return state[u]; },
+                m_all, l_all, count - s0, [&](int u) __attribute__((always_inline)) { return state[u]; },
                 [&](int u, PartWeights w) __attribute__((always_inline)) {
 #pragma unroll
                     for (int x = 0; x < kPasses; ++x) sum[x] = merged(sum[x], part[u][x], w);
@@ -739,11 +811,11 @@ extern "C" int tilemix_attention_cache4(const TileMixCache4AttentionArgs* args, 
     p.negate = a.score_scale < 0.0f;
     // (Of a score_scale of 0 the smallest number: a hidden token's -inf times it is still -inf.)
     p.score_log2 = std::max(std::fabs(a.score_scale) * kLog2e, FLT_MIN);
-    // Ranges of at least kLeastSteps blocks.
     const std::int64_t items = static_cast<std::int64_t>(a.batch) * a.kv_heads * p.tiles;
-    const std::int64_t most = (p.most_tokens - 1) / kCacheKeys + 1;  // blocks of one of them
-    const int ranges = p.group <= 8 ? kRanges : kRanges16;
-    p.ranges = static_cast<int>(std::min<std::int64_t>(ranges, items > ranges * kLeastSteps ? ranges : (items * most - 1) / kLeastSteps + 1));
+    // Places of one of them, and its end rounded up to a range's length.
+    const std::int64_t most = 2 * ((p.most_tokens - 1) / kCacheKeys + 1 + kSwitch);
+    if (items > 0x3fffffffLL / most) return hipErrorInvalidConfiguration;
+    p.ranges = static_cast<int>(std::min<std::int64_t>(kRanges, (items * most - 1) / kLeastSteps + 1));
     const hipError_t found = check_device();
     if (found != hipSuccess) return found;
     const hipStream_t s = static_cast<hipStream_t>(stream);
