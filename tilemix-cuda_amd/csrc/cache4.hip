@@ -39,8 +39,6 @@ struct AppendParams {
     int tokens, positions;
     int q_heads, kv_heads;
     int d, rotary, half;
-    int interleaved;
-    int vector_partner;  // half is a multiple of 8
     int heads_per_wave;
 };
 
@@ -104,7 +102,12 @@ __device__ __forceinline__ uint4v pack8(const float (&x)[8]) {
                   pack_pair<kBf16>(x[6], x[7])};
 }
 
-template <int kGroups, bool kBf16>
+// How features are turned: not at all; with the feature half the turned ones away, in
+// 16-byte pieces or one by one; with their neighbours.
+enum class Turn { kNone, kHalves, kHalvesSingle, kPairs };
+enum class Kind { kQuery, kKey, kValue };
+
+template <int kGroups, bool kBf16, Turn kTurn>
 __global__ __launch_bounds__(kCacheThreads) void cache4_append_kernel(const AppendParams p) {
     constexpr int kTeam = 8 * kGroups;
     constexpr int kTokens = kWave / kTeam;  // of a workgroup
@@ -113,29 +116,41 @@ __global__ __launch_bounds__(kCacheThreads) void cache4_append_kernel(const Appe
     const int token = blockIdx.x * kTokens + lane / kTeam;
     const int chunk = lane % kTeam;  // of 8 features
     const int f0 = 8 * chunk;
-    const int d = p.d;
+    const int first = (blockIdx.y * kCacheWaves + wave) * p.heads_per_wave;
+    const int last = min(first + p.heads_per_wave, p.q_heads + 2 * p.kv_heads);
 
     bool valid = token < p.tokens;  // and its position is in the table
     Place at{0, 0, false};
     float cosine[8], sine[8];  // per feature: y = x cosine + partner sine, the sign in the sine
-    const bool turned = f0 < p.rotary;
-    int partner = f0;  // first feature of the partners (vector_partner)
-    if (turned && !p.interleaved) partner = f0 < p.half ? f0 + p.half : f0 - p.half;
-#pragma unroll
-    for (int e = 0; e < 8; ++e) cosine[e] = 1.0f, sine[e] = 0.0f;
+    const bool turned = kTurn != Turn::kNone && f0 < p.rotary;
+    const bool second_half = f0 >= p.half;  // (kHalves)
+    const int partner = second_half ? f0 - p.half : f0 + p.half;
     if (valid) {
         at = place_of(p.cache, p.slots[token]);
-        if (p.rotary > 0) {
+        if constexpr (kTurn != Turn::kNone) {
             const int position = p.token_positions[token];
             valid = position >= 0 && position < p.positions;
             const float* const row = p.cos_sin + static_cast<std::int64_t>(valid ? position : 0) * p.rotary;
-            if (valid) {
+            if constexpr (kTurn == Turn::kHalves) {
+                if (turned) {
+                    const float* const from = row + (second_half ? partner : f0);
+                    const float flip = second_half ? 1.0f : -1.0f;
+#pragma unroll
+                    for (int x = 0; x < 2; ++x) {
+                        const float4v c = *reinterpret_cast<const float4v*>(from + 4 * x);
+                        const float4v s = *reinterpret_cast<const float4v*>(from + p.half + 4 * x);
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) cosine[4 * x + e] = c[e], sine[4 * x + e] = s[e] * flip;
+                    }
+                }
+            } else {
 #pragma unroll
                 for (int e = 0; e < 8; ++e) {
                     const int f = f0 + e;
+                    cosine[e] = 1.0f, sine[e] = 0.0f;
                     if (f < p.rotary) {
-                        const bool second = p.interleaved ? f & 1 : f >= p.half;
-                        const int angle = p.interleaved ? f >> 1 : second ? f - p.half : f;
+                        const bool second = kTurn == Turn::kPairs ? f & 1 : f >= p.half;
+                        const int angle = kTurn == Turn::kPairs ? f >> 1 : second ? f - p.half : f;
                         cosine[e] = row[angle];
                         sine[e] = second ? row[p.half + angle] : -row[p.half + angle];
                     }
@@ -143,122 +158,117 @@ __global__ __launch_bounds__(kCacheThreads) void cache4_append_kernel(const Appe
             }
         }
     }
-    const bool live = valid && f0 < d;     // holds values
-    const bool cached = valid && at.ok;    // writes to the cache, code 0 past d
+    const bool live = valid && f0 < p.d;  // holds values
+    const bool cached = valid && at.ok;   // writes to the cache, code 0 past d
     const int place = cache_place(at.t);
+    std::uint8_t* const head0_block = p.cache.data + at.block;
 
-    const int first = (blockIdx.y * kCacheWaves + wave) * p.heads_per_wave;
-    const int last = min(first + p.heads_per_wave, p.q_heads + 2 * p.kv_heads);
-    // Rows of queries, then keys, then values.
-    enum Kind { kQuery, kKey, kValue };
-    struct Head {
-        TokenRows rows;
-        int index;
-        Kind kind;
-    };
-    auto head_at = [&](int n) __attribute__((always_inline)) {
-        if (n < p.q_heads) return Head{p.q, n, kQuery};
-        if (n < p.q_heads + p.kv_heads) return Head{p.k, n - p.q_heads, kKey};
-        return Head{p.v, n - p.q_heads - p.kv_heads, kValue};
-    };
-    struct Row {
-        uint4v own, other;
-    };
-    auto load = [&](int n) __attribute__((always_inline)) {
-        Row row{};
-        const Head head = head_at(n);
-        if (live) {
-            const std::uint16_t* const x = head.rows.in + token * head.rows.in_rows.row + head.index * head.rows.in_rows.head;
-            row.own = *reinterpret_cast<const uint4v*>(x + f0);
-            if (head.kind != kValue && turned && p.vector_partner) row.other = *reinterpret_cast<const uint4v*>(x + partner);
-        }
-        return row;
-    };
-    auto take = [&](int n, const Row& row) __attribute__((always_inline)) {
-        const Head head = head_at(n);
-        float x[8];
-        unpack8<kBf16>(row.own, x);
-        if (head.kind != kValue && p.rotary > 0) {
-            float other[8];
-            if (p.interleaved) {
+    // Rows from .. to - 1 of one kind, kBatch of them loaded before the first is taken.
+    auto rows_of = [&](auto kind, const TokenRows& rows, int from, int to) __attribute__((always_inline)) {
+        constexpr Kind kKind = decltype(kind)::value;
+        constexpr bool kTurned = kTurn != Turn::kNone && kKind != Kind::kValue;
+        constexpr int kBatch = 4;
+        const std::uint16_t* const in = rows.in + token * rows.in_rows.row + f0;
+        std::uint16_t* const out = rows.out + token * rows.out_rows.row + f0;
+        for (int head = from; head < to; head += kBatch) {
+            uint4v own[kBatch], other[kBatch];
 #pragma unroll
-                for (int e = 0; e < 8; ++e) other[e] = x[e ^ 1];
-            } else if (p.vector_partner) {
-                unpack8<kBf16>(row.other, other);
-            } else {
-                const std::uint16_t* const in = head.rows.in + token * head.rows.in_rows.row + head.index * head.rows.in_rows.head;
-#pragma unroll
-                for (int e = 0; e < 8; ++e) {
-                    const int f = f0 + e;
-                    other[e] = live && f < p.rotary ? half_of<kBf16, 0>(in[f < p.half ? f + p.half : f - p.half]) : 0.0f;
+            for (int b = 0; b < kBatch; ++b) {
+                own[b] = other[b] = uint4v{0u, 0u, 0u, 0u};
+                if (live && head + b < to) {
+                    const std::uint16_t* const x = in + (head + b) * rows.in_rows.head;
+                    own[b] = *reinterpret_cast<const uint4v*>(x);
+                    if constexpr (kTurned && kTurn == Turn::kHalves)
+                        if (turned) other[b] = *reinterpret_cast<const uint4v*>(x + (partner - f0));
                 }
             }
 #pragma unroll
-            for (int e = 0; e < 8; ++e)
-                if (f0 + e < p.rotary) x[e] = rounded_product(x[e], cosine[e]) + rounded_product(other[e], sine[e]);
-        }
-        if (head.rows.out && live) {
-            std::uint16_t* const y = head.rows.out + token * head.rows.out_rows.row + head.index * head.rows.out_rows.head;
-            *reinterpret_cast<uint4v*>(y + f0) = pack8<kBf16>(x);
-        }
-        if (head.kind == kQuery) return;
-        // Extremes of the group; `zero` becomes NaN with any value that is not finite.
-        float low = INFINITY, high = -INFINITY, zero = 0.0f;
-        if (live) {
+            for (int b = 0; b < kBatch; ++b) {
+                if (head + b >= to) break;
+                float x[8];
+                unpack8<kBf16>(own[b], x);
+                if constexpr (kTurned) {
+                    float partners[8];
+                    if constexpr (kTurn == Turn::kHalves) {
+                        unpack8<kBf16>(other[b], partners);
+                    } else if constexpr (kTurn == Turn::kPairs) {
 #pragma unroll
-            for (int e = 0; e < 8; ++e) {
-                low = fminf(low, x[e]);
-                high = fmaxf(high, x[e]);
-                zero = __builtin_fmaf(x[e], 0.0f, zero);
+                        for (int e = 0; e < 8; ++e) partners[e] = x[e ^ 1];
+                    } else {
+                        const std::uint16_t* const row = in + (head + b) * rows.in_rows.head - f0;
+#pragma unroll
+                        for (int e = 0; e < 8; ++e) {
+                            const int f = f0 + e;
+                            partners[e] = live && f < p.rotary ? half_of<kBf16, 0>(row[f < p.half ? f + p.half : f - p.half]) : 0.0f;
+                        }
+                    }
+#pragma unroll
+                    for (int e = 0; e < 8; ++e)
+                        if (kTurn == Turn::kHalves ? turned : f0 + e < p.rotary)
+                            x[e] = rounded_product(x[e], cosine[e]) + rounded_product(partners[e], sine[e]);
+                }
+                if (kKind != Kind::kValue && rows.out && live)
+                    *reinterpret_cast<uint4v*>(out + (head + b) * rows.out_rows.head) = pack8<kBf16>(x);
+                if constexpr (kKind == Kind::kQuery) continue;
+                // Extremes of the group; `zero` becomes NaN with any value that is not finite.
+                float low = live ? x[0] : INFINITY, high = live ? x[0] : -INFINITY, zero = live ? x[0] * 0.0f : 0.0f;
+                if (live) {
+#pragma unroll
+                    for (int e = 1; e < 8; ++e) {
+                        low = fminf(low, x[e]);
+                        high = fmaxf(high, x[e]);
+                        zero = __builtin_fmaf(x[e], 0.0f, zero);
+                    }
+                }
+                low = over_8_lanes(low, [](float a, float b) { return fminf(a, b); });
+                high = over_8_lanes(high, [](float a, float b) { return fmaxf(a, b); });
+                zero = over_8_lanes(zero, [](float a, float b) { return a + b; });
+                const float minimum = half_of<true, 1>(pack_pair<true>(0.0f, low)) + 0.0f;  // a zero without its sign
+                std::uint32_t params = pack_pair<true>((high - minimum) / 15.0f, minimum);
+                const float scale = half_of<true, 0>(params);
+                const bool finite = zero == 0.0f && scale < INFINITY;
+                const bool coded = finite && scale >= kLeastScale;
+                if (!finite) params = 0x7fc07fc0u;
+                else if (!coded) params &= 0xffff0000u;
+                const float recip = 1.0f / scale;
+                std::uint32_t code[8];
+#pragma unroll
+                for (int e = 0; e < 8; ++e)
+                    code[e] = static_cast<std::uint32_t>(
+                        __builtin_amdgcn_fmed3f(__builtin_rintf(quotient(x[e] - minimum, scale, recip)), 0.0f, 15.0f));
+                const bool written = coded && live;
+                if (cached) {
+                    std::uint8_t* const block = head0_block + (head + b) * p.cache.head_bytes;
+                    if constexpr (kKind == Kind::kKey) {
+                        std::uint32_t word = 0;
+#pragma unroll
+                        for (int e = 0; e < 8; ++e) word |= code[e] << (4 * (e / 2) + 16 * (e % 2));
+                        const int m = chunk >> 3, g = (chunk >> 1) & 3, w = chunk & 1;
+                        reinterpret_cast<std::uint32_t*>(block)[8 * kGroups * at.t + 2 * kGroups * g + 2 * m + w] = written ? word : 0u;
+                    } else {
+                        auto* const quarters = reinterpret_cast<std::uint16_t*>(block + cache_values_at(kGroups)) + place;
+#pragma unroll
+                        for (int half = 0; half < 2; ++half) {
+                            const std::uint32_t word = code[4 * half] | (code[4 * half + 1] << 4) | (code[4 * half + 2] << 8) |
+                                                       (code[4 * half + 3] << 12);
+                            quarters[(2 * chunk + half) * kCacheKeys] = static_cast<std::uint16_t>(written ? word : 0u);
+                        }
+                    }
+                    if ((chunk & 7) == 0)
+                        reinterpret_cast<std::uint32_t*>(
+                            block + (kKind == Kind::kKey ? cache_key_params_at(kGroups) : cache_value_params_at(kGroups)))
+                            [(chunk >> 3) * kCacheKeys + place] = params;
+                }
             }
         }
-        low = over_8_lanes(low, [](float a, float b) { return fminf(a, b); });
-        high = over_8_lanes(high, [](float a, float b) { return fmaxf(a, b); });
-        zero = over_8_lanes(zero, [](float a, float b) { return a + b; });
-        const float minimum = half_of<true, 1>(pack_pair<true>(0.0f, low)) + 0.0f;  // a zero without its sign
-        std::uint32_t params = pack_pair<true>((high - minimum) / 15.0f, minimum);
-        const float scale = half_of<true, 0>(params);
-        const bool finite = zero == 0.0f && scale < INFINITY;
-        const bool coded = finite && scale >= kLeastScale;
-        if (!finite) params = 0x7fc07fc0u;
-        else if (!coded) params &= 0xffff0000u;
-        const float recip = 1.0f / scale;
-        std::uint32_t code[8];
-#pragma unroll
-        for (int e = 0; e < 8; ++e) {
-            const float steps = __builtin_rintf(quotient(x[e] - minimum, scale, recip));
-            code[e] = coded && live ? static_cast<std::uint32_t>(fminf(fmaxf(steps, 0.0f), 15.0f)) : 0u;
-        }
-        if (!cached) return;
-        std::uint8_t* const block = p.cache.data + at.block + head.index * p.cache.head_bytes;
-        if (head.kind == kKey) {
-            std::uint32_t word = 0;
-#pragma unroll
-            for (int e = 0; e < 8; ++e) word |= code[e] << (4 * (e / 2) + 16 * (e % 2));
-            const int m = chunk >> 3, g = (chunk >> 1) & 3, w = chunk & 1;
-            reinterpret_cast<std::uint32_t*>(block)[8 * kGroups * at.t + 2 * kGroups * g + 2 * m + w] = word;
-        } else {
-            auto* const quarters = reinterpret_cast<std::uint16_t*>(block + cache_values_at(kGroups)) + place;
-#pragma unroll
-            for (int half = 0; half < 2; ++half)
-                quarters[(2 * chunk + half) * kCacheKeys] =
-                    static_cast<std::uint16_t>(code[4 * half] | (code[4 * half + 1] << 4) | (code[4 * half + 2] << 8) |
-                                               (code[4 * half + 3] << 12));
-        }
-        if ((chunk & 7) == 0)
-            reinterpret_cast<std::uint32_t*>(block + (head.kind == kKey ? cache_key_params_at(kGroups) : cache_value_params_at(kGroups)))
-                [(chunk >> 3) * kCacheKeys + place] = params;
     };
-    constexpr int kBatch = 4;
-    for (int n = first; n < last; n += kBatch) {
-        Row rows[kBatch];
-#pragma unroll
-        for (int b = 0; b < kBatch; ++b)
-            if (n + b < last) rows[b] = load(n + b);
-#pragma unroll
-        for (int b = 0; b < kBatch; ++b)
-            if (n + b < last) take(n + b, rows[b]);
-    }
+    using Query = std::integral_constant<Kind, Kind::kQuery>;
+    using Key = std::integral_constant<Kind, Kind::kKey>;
+    using Value = std::integral_constant<Kind, Kind::kValue>;
+    const int keys = p.q_heads, values = keys + p.kv_heads;  // queries, then keys, then values
+    rows_of(Query{}, p.q, first, min(last, keys));
+    rows_of(Key{}, p.k, max(first - keys, 0), min(last, values) - keys);
+    rows_of(Value{}, p.v, max(first - values, 0), last - values);
 }
 
 template <int kGroups, bool kBf16>
@@ -274,59 +284,55 @@ __global__ __launch_bounds__(kCacheThreads) void cache4_gather_kernel(const Gath
     if (!at.ok) return;
     const int place = cache_place(at.t);
     const int m = chunk >> 3, g = (chunk >> 1) & 3, w = chunk & 1;
-    const int heads_k = p.k.out ? p.kv_heads : 0, heads = heads_k + (p.v.out ? p.kv_heads : 0);
+    const int keys = p.k.out ? p.kv_heads : 0, heads = keys + (p.v.out ? p.kv_heads : 0);
     const int first = (blockIdx.y * kCacheWaves + wave) * p.heads_per_wave;
     const int last = min(first + p.heads_per_wave, heads);
-    struct Codes {
-        std::uint32_t params, low, high;  // a key's word is in low
-    };
-    auto load = [&](int n) __attribute__((always_inline)) {
-        const bool key = n < heads_k;
-        const std::uint8_t* const block = p.cache.data + at.block + (key ? n : n - heads_k) * p.cache.head_bytes;
-        Codes c{};
-        if (key) {
-            c.low = reinterpret_cast<const std::uint32_t*>(block)[8 * kGroups * at.t + 2 * kGroups * g + 2 * m + w];
-        } else {
-            const auto* const quarters = reinterpret_cast<const std::uint16_t*>(block + cache_values_at(kGroups)) + place;
-            c.low = quarters[2 * chunk * kCacheKeys];
-            c.high = quarters[(2 * chunk + 1) * kCacheKeys];
+    const std::uint8_t* const head0_block = p.cache.data + at.block;
+    auto rows_of = [&](auto kind, const TokenRows& rows, int from, int to) __attribute__((always_inline)) {
+        constexpr bool kKey = decltype(kind)::value == Kind::kKey;
+        constexpr int kBatch = 4;
+        std::uint16_t* const out = rows.out + token * rows.out_rows.row + f0;
+        for (int head = from; head < to; head += kBatch) {
+            std::uint32_t params[kBatch], codes[kBatch][2];
+#pragma unroll
+            for (int b = 0; b < kBatch; ++b) {
+                const std::uint8_t* const block = head0_block + min(head + b, to - 1) * p.cache.head_bytes;
+                params[b] = reinterpret_cast<const std::uint32_t*>(
+                    block + (kKey ? cache_key_params_at(kGroups) : cache_value_params_at(kGroups)))[m * kCacheKeys + place];
+                if constexpr (kKey) {
+                    codes[b][0] = reinterpret_cast<const std::uint32_t*>(block)[8 * kGroups * at.t + 2 * kGroups * g + 2 * m + w];
+                } else {
+                    const auto* const quarters = reinterpret_cast<const std::uint16_t*>(block + cache_values_at(kGroups)) + place;
+#pragma unroll
+                    for (int half = 0; half < 2; ++half) codes[b][half] = quarters[(2 * chunk + half) * kCacheKeys];
+                }
+            }
+#pragma unroll
+            for (int b = 0; b < kBatch; ++b) {
+                if (head + b >= to) break;
+                const float scale = half_of<true, 0>(params[b]), minimum = half_of<true, 1>(params[b]);
+                float x[8];
+#pragma unroll
+                for (int e = 0; e < 8; ++e) {
+                    const std::uint32_t code = kKey ? codes[b][0] >> (4 * (e / 2) + 16 * (e % 2)) : codes[b][e / 4] >> (4 * (e % 4));
+                    x[e] = __builtin_fmaf(scale, static_cast<float>(code & 15u), minimum);
+                }
+                *reinterpret_cast<uint4v*>(out + (head + b) * rows.out_rows.head) = pack8<kBf16>(x);
+            }
         }
-        c.params = reinterpret_cast<const std::uint32_t*>(
-            block + (key ? cache_key_params_at(kGroups) : cache_value_params_at(kGroups)))[m * kCacheKeys + place];
-        return c;
     };
-    auto take = [&](int n, const Codes& c) __attribute__((always_inline)) {
-        const bool key = n < heads_k;
-        const TokenRows rows = key ? p.k : p.v;
-        const float scale = half_of<true, 0>(c.params), minimum = half_of<true, 1>(c.params);
-        float x[8];
-#pragma unroll
-        for (int e = 0; e < 8; ++e) {
-            const std::uint32_t code = key ? c.low >> (4 * (e / 2) + 16 * (e % 2)) : (e < 4 ? c.low : c.high) >> (4 * (e % 4));
-            x[e] = __builtin_fmaf(scale, static_cast<float>(code & 15u), minimum);
-        }
-        std::uint16_t* const y = rows.out + token * rows.out_rows.row + (key ? n : n - heads_k) * rows.out_rows.head;
-        *reinterpret_cast<uint4v*>(y + f0) = pack8<kBf16>(x);
-    };
-    constexpr int kBatch = 4;
-    for (int n = first; n < last; n += kBatch) {
-        Codes codes[kBatch];
-#pragma unroll
-        for (int b = 0; b < kBatch; ++b)
-            if (n + b < last) codes[b] = load(n + b);
-#pragma unroll
-        for (int b = 0; b < kBatch; ++b)
-            if (n + b < last) take(n + b, codes[b]);
-    }
+    rows_of(std::integral_constant<Kind, Kind::kKey>{}, p.k, first, min(last, keys));
+    rows_of(std::integral_constant<Kind, Kind::kValue>{}, p.v, max(first - keys, 0), last - keys);
 }
 
-// Heads that one wave takes in turn: enough waves to fill the device first.
+// Heads that one wave takes in turn: enough waves to fill the device first, then the
+// fewest that let a workgroup's waves have all of them.
 int heads_per_wave(std::int64_t token_groups, int heads) {
-    constexpr int kWavesWanted = 4096, kMost = 16;
-    return static_cast<int>(std::clamp<std::int64_t>(token_groups * heads / kWavesWanted, 1, std::min(heads, kMost)));
+    constexpr int kWavesWanted = 4096;
+    return static_cast<int>(std::clamp<std::int64_t>(token_groups * heads / kWavesWanted, 1, (heads - 1) / kCacheWaves + 1));
 }
 
-template <int kGroups>
+template <int kGroups, Turn kTurn>
 hipError_t launch_append(AppendParams p, bool bf16, hipStream_t stream) {
     constexpr int kTokens = kWave / (8 * kGroups);
     const unsigned token_groups = static_cast<unsigned>((p.tokens - 1) / kTokens + 1);
@@ -336,10 +342,15 @@ hipError_t launch_append(AppendParams p, bool bf16, hipStream_t stream) {
     const dim3 grid(token_groups, static_cast<unsigned>((heads + per_group - 1) / per_group));
     if (grid.y > 65535) return hipErrorInvalidConfiguration;
     if (bf16)
-        cache4_append_kernel<kGroups, true><<<grid, kCacheThreads, 0, stream>>>(p);
+        cache4_append_kernel<kGroups, true, kTurn><<<grid, kCacheThreads, 0, stream>>>(p);
     else
-        cache4_append_kernel<kGroups, false><<<grid, kCacheThreads, 0, stream>>>(p);
+        cache4_append_kernel<kGroups, false, kTurn><<<grid, kCacheThreads, 0, stream>>>(p);
     return hipGetLastError();
+}
+
+template <Turn kTurn>
+hipError_t launch_append(const AppendParams& p, bool bf16, hipStream_t stream) {
+    return p.cache.groups == 1 ? launch_append<1, kTurn>(p, bf16, stream) : launch_append<2, kTurn>(p, bf16, stream);
 }
 
 template <int kGroups>
@@ -408,13 +419,14 @@ extern "C" int tilemix_cache4_append(const TileMixCache4AppendArgs* args, void* 
     p.d = a.d;
     p.rotary = a.rotary_dim;
     p.half = a.rotary_dim / 2;
-    p.interleaved = a.interleaved != 0;
-    p.vector_partner = !p.interleaved && p.half % 8 == 0;
     const hipError_t found = check_device();
     if (found != hipSuccess) return found;
     const bool bf16 = a.dtype == TILEMIX_DTYPE_BF16;
-    return p.cache.groups == 1 ? launch_append<1>(p, bf16, static_cast<hipStream_t>(stream))
-                               : launch_append<2>(p, bf16, static_cast<hipStream_t>(stream));
+    const hipStream_t s = static_cast<hipStream_t>(stream);
+    if (p.rotary == 0) return launch_append<Turn::kNone>(p, bf16, s);
+    if (a.interleaved) return launch_append<Turn::kPairs>(p, bf16, s);
+    const bool pieces = p.half % 8 == 0 && reinterpret_cast<std::uintptr_t>(p.cos_sin) % 16 == 0;
+    return pieces ? launch_append<Turn::kHalves>(p, bf16, s) : launch_append<Turn::kHalvesSingle>(p, bf16, s);
 }
 
 extern "C" int tilemix_cache4_gather(const TileMixCache4GatherArgs* args, void* stream) {
