@@ -9,8 +9,11 @@
 // of 8; else single values) and a group's extremes are three DPP steps. The teams of
 // a wave hold consecutive tokens of the same head: their key codes are one run of
 // the block, and their 16-bit pieces of a value row lie side by side, so that a
-// store touches 8 bytes of each line instead of 2. The waves of a workgroup take
-// different heads of the same tokens, with the cosines and sines kept in registers.
+// store touches 8 bytes of each line instead of 2. The waves of a workgroup take the
+// tokens after one another's, for the same reason, and workgroups that share a block of
+// the cache run on one XCD (token_group_of): dealt out one by one, eight L2s would each
+// read, or write a piece of, the same lines. A wave takes several heads with the
+// cosines and sines kept in registers.
 
 #include "serving.h"
 #include "tilemix_capi.h"
@@ -23,6 +26,7 @@ namespace {
 
 constexpr int kCacheThreads = 256;
 constexpr int kCacheWaves = kCacheThreads / kWave;
+constexpr int kXcds = 8;
 
 struct TokenRows {
     const std::uint16_t* in;
@@ -62,6 +66,12 @@ __device__ __forceinline__ float over_8_lanes(float x, F&& f) {
     x = f(x, step(std::integral_constant<int, 0xb1>{}));   // lane ^ 1
     x = f(x, step(std::integral_constant<int, 0x4e>{}));   // lane ^ 2
     return f(x, step(std::integral_constant<int, 0x141>{}));  // mirrored within 8
+}
+
+// Token group (the tokens of a wave) of wave `wave` of workgroup `x` of `count`, a multiple
+// of 8: workgroups are dealt round-robin to the 8 XCDs, each of which takes a run.
+__device__ __forceinline__ int token_group_of(int x, int count, int wave) {
+    return (x % kXcds * (count / kXcds) + x / kXcds) * kCacheWaves + wave;
 }
 
 // Where the cache has a slot: byte offset of head 0's block and the token's number in it.
@@ -110,13 +120,13 @@ enum class Kind { kQuery, kKey, kValue };
 template <int kGroups, bool kBf16, Turn kTurn>
 __global__ __launch_bounds__(kCacheThreads) void cache4_append_kernel(const AppendParams p) {
     constexpr int kTeam = 8 * kGroups;
-    constexpr int kTokens = kWave / kTeam;  // of a workgroup
+    constexpr int kTokens = kWave / kTeam;  // of a wave
     const int lane = threadIdx.x & (kWave - 1);
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int token = blockIdx.x * kTokens + lane / kTeam;
+    const int token = token_group_of(blockIdx.x, gridDim.x, wave) * kTokens + lane / kTeam;
     const int chunk = lane % kTeam;  // of 8 features
     const int f0 = 8 * chunk;
-    const int first = (blockIdx.y * kCacheWaves + wave) * p.heads_per_wave;
+    const int first = blockIdx.y * p.heads_per_wave;
     const int last = min(first + p.heads_per_wave, p.q_heads + 2 * p.kv_heads);
 
     bool valid = token < p.tokens;  // and its position is in the table
@@ -277,7 +287,7 @@ __global__ __launch_bounds__(kCacheThreads) void cache4_gather_kernel(const Gath
     constexpr int kTokens = kWave / kTeam;
     const int lane = threadIdx.x & (kWave - 1);
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int token = blockIdx.x * kTokens + lane / kTeam;
+    const int token = token_group_of(blockIdx.x, gridDim.x, wave) * kTokens + lane / kTeam;
     const int chunk = lane % kTeam, f0 = 8 * chunk;
     if (token >= p.tokens || f0 >= p.d) return;
     const Place at = place_of(p.cache, p.slots[token]);
@@ -285,7 +295,7 @@ __global__ __launch_bounds__(kCacheThreads) void cache4_gather_kernel(const Gath
     const int place = cache_place(at.t);
     const int m = chunk >> 3, g = (chunk >> 1) & 3, w = chunk & 1;
     const int keys = p.k.out ? p.kv_heads : 0, heads = keys + (p.v.out ? p.kv_heads : 0);
-    const int first = (blockIdx.y * kCacheWaves + wave) * p.heads_per_wave;
+    const int first = blockIdx.y * p.heads_per_wave;
     const int last = min(first + p.heads_per_wave, heads);
     const std::uint8_t* const head0_block = p.cache.data + at.block;
     auto rows_of = [&](auto kind, const TokenRows& rows, int from, int to) __attribute__((always_inline)) {
@@ -325,22 +335,22 @@ __global__ __launch_bounds__(kCacheThreads) void cache4_gather_kernel(const Gath
     rows_of(std::integral_constant<Kind, Kind::kValue>{}, p.v, max(first - keys, 0), last - keys);
 }
 
-// Heads that one wave takes in turn: enough waves to fill the device first, then the
-// fewest that let a workgroup's waves have all of them.
-int heads_per_wave(std::int64_t token_groups, int heads) {
+// Heads that one wave takes in turn, and the grid: enough waves to fill the device.
+hipError_t plan_rows(int tokens, int tokens_per_wave, int heads, int& heads_per_wave, dim3& grid) {
     constexpr int kWavesWanted = 4096;
-    return static_cast<int>(std::clamp<std::int64_t>(token_groups * heads / kWavesWanted, 1, (heads - 1) / kCacheWaves + 1));
+    const std::int64_t token_groups = (tokens - 1) / tokens_per_wave + 1;
+    heads_per_wave = static_cast<int>(std::clamp<std::int64_t>(token_groups * heads / kWavesWanted, 1, heads));
+    const std::int64_t workgroups = (token_groups - 1) / kCacheWaves + 1;
+    grid = dim3(static_cast<unsigned>((workgroups + kXcds - 1) / kXcds * kXcds),
+                static_cast<unsigned>((heads - 1) / heads_per_wave + 1));
+    return grid.y > 65535 ? hipErrorInvalidConfiguration : hipSuccess;
 }
 
 template <int kGroups, Turn kTurn>
 hipError_t launch_append(AppendParams p, bool bf16, hipStream_t stream) {
-    constexpr int kTokens = kWave / (8 * kGroups);
-    const unsigned token_groups = static_cast<unsigned>((p.tokens - 1) / kTokens + 1);
-    const int heads = p.q_heads + 2 * p.kv_heads;
-    p.heads_per_wave = heads_per_wave(token_groups, heads);
-    const int per_group = kCacheWaves * p.heads_per_wave;
-    const dim3 grid(token_groups, static_cast<unsigned>((heads + per_group - 1) / per_group));
-    if (grid.y > 65535) return hipErrorInvalidConfiguration;
+    dim3 grid;
+    const hipError_t planned = plan_rows(p.tokens, kWave / (8 * kGroups), p.q_heads + 2 * p.kv_heads, p.heads_per_wave, grid);
+    if (planned != hipSuccess) return planned;
     if (bf16)
         cache4_append_kernel<kGroups, true, kTurn><<<grid, kCacheThreads, 0, stream>>>(p);
     else
@@ -355,13 +365,10 @@ hipError_t launch_append(const AppendParams& p, bool bf16, hipStream_t stream) {
 
 template <int kGroups>
 hipError_t launch_gather(GatherParams p, bool bf16, hipStream_t stream) {
-    constexpr int kTokens = kWave / (8 * kGroups);
-    const unsigned token_groups = static_cast<unsigned>((p.tokens - 1) / kTokens + 1);
-    const int heads = (p.k.out ? p.kv_heads : 0) + (p.v.out ? p.kv_heads : 0);
-    p.heads_per_wave = heads_per_wave(token_groups, heads);
-    const int per_group = kCacheWaves * p.heads_per_wave;
-    const dim3 grid(token_groups, static_cast<unsigned>((heads + per_group - 1) / per_group));
-    if (grid.y > 65535) return hipErrorInvalidConfiguration;
+    dim3 grid;
+    const hipError_t planned =
+        plan_rows(p.tokens, kWave / (8 * kGroups), (p.k.out ? p.kv_heads : 0) + (p.v.out ? p.kv_heads : 0), p.heads_per_wave, grid);
+    if (planned != hipSuccess) return planned;
     if (bf16)
         cache4_gather_kernel<kGroups, true><<<grid, kCacheThreads, 0, stream>>>(p);
     else
