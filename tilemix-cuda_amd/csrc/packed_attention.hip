@@ -221,25 +221,23 @@ __device__ __forceinline__ bool not_finite(uint4v v) {
     return any;
 }
 
-// What P.V takes of a value that is not finite, per half: class 0 the finite
-// values (others 0), 1 one for +inf, 2 one for -inf, 3 one for NaN.
+// 8-bit masks (bit e: half e) of the +inf, -inf and NaN values of a fragment, which become
+// 0 in it.
 template <bool kBf16>
-__device__ __forceinline__ uint4v value_class(uint4v v, int which) {
-    constexpr unsigned kExponent = kBf16 ? 0x7f80u : 0x7c00u, kOne = kBf16 ? 0x3f80u : 0x3c00u;
-    uint4v out;
+__device__ __forceinline__ uint4v take_out_special(uint4v v, unsigned (&masks)[3]) {
+    constexpr unsigned kExponent = kBf16 ? 0x7f80u : 0x7c00u;
+    masks[0] = masks[1] = masks[2] = 0;
 #pragma unroll
-    for (int w = 0; w < 4; ++w) {
-        unsigned word = 0;
+    for (int e = 0; e < 8; ++e) {
+        const unsigned x = (v[e / 2] >> (16 * (e % 2))) & 0xffffu, magnitude = x & 0x7fffu;
+        if (magnitude >= kExponent) {
+            const int kind = magnitude > kExponent ? 2 : static_cast<int>(x >> 15);
 #pragma unroll
-        for (int half = 0; half < 2; ++half) {
-            const unsigned x = (v[w] >> (16 * half)) & 0xffffu, magnitude = x & 0x7fffu;
-            const unsigned kind = magnitude < kExponent ? 0u : magnitude > kExponent ? 3u : 1u + (x >> 15);
-            const unsigned value = kind != static_cast<unsigned>(which) ? 0u : which == 0 ? x : kOne;
-            word |= value << (16 * half);
+            for (int k = 0; k < 3; ++k) masks[k] |= (kind == k ? 1u : 0u) << e;
+            v[e / 2] &= e % 2 ? 0x0000ffffu : 0xffff0000u;
         }
-        out[w] = word;
     }
-    return out;
+    return v;
 }
 
 template <int DC, bool kBf16>
@@ -251,6 +249,11 @@ __global__ __launch_bounds__(kThreadsPerGroup, 2) void packed_attention_kernel(c
     // K | V 0 | V 1
     __shared__ __attribute__((aligned(16))) unsigned char smem[L::kKBytes + 2 * L::kVBytes];
     __shared__ __attribute__((aligned(16))) unsigned char lds_spare[1024];  // landing area of the spare DMA slots
+    // Which values of a diagonal tile are +inf, -inf and NaN, a byte for each 16-byte chunk; and
+    // the last tile (counted from 1) that has any.
+    constexpr int kChunks = kDP / 8;
+    __shared__ __attribute__((aligned(16))) unsigned char lds_special[3][kTileKeys * kChunks];
+    __shared__ int lds_special_tile;
     unsigned char* const lds_k = smem;
     unsigned char* const lds_v = smem + L::kKBytes;
     const unsigned lds_k_address = lds_address_of(smem);
@@ -362,6 +365,11 @@ __global__ __launch_bounds__(kThreadsPerGroup, 2) void packed_attention_kernel(c
     const int wave_last = tw >= seq.q_len ? -1 : p.causal ? min(context + tw + kRowsPerWave, seq.k_len) - 1 : seq.k_len - 1;
     const int all_last = p.causal ? context + tw : seq.k_len - 1;
 
+    // A row's probability of a key that it does not see is 0, but 0 times an infinite or NaN
+    // value is NaN: such values are taken out of diagonal tiles, and put into the rows that
+    // see them afterwards.
+    const int first_hidden = p.causal ? context + t0 + 1 : seq.k_len;  // first key that some row of the workgroup does not see
+    if (tid == 0) lds_special_tile = 0;
     int v_buffer = 0;
     if (tiles > 0) {
         issue_k(0);
@@ -405,8 +413,34 @@ __global__ __launch_bounds__(kThreadsPerGroup, 2) void packed_attention_kernel(c
                     s[kb][e] = 32 * kb + 8 * (e >> 2) + (e & 3) > seen ? -INFINITY : s[kb][e] * c;
             c = 1.0f;
         }
+        const bool diagonal = k0 + kTileKeys > first_hidden;  // of the workgroup
+        unsigned char* const v_tile = lds_v + (v_buffer ? L::kVBytes : 0);
+        constexpr int kChecks = kTileKeys * kChunks / kThreadsPerGroup;  // chunks of a thread
+        auto checked = [&](int x) {
+            const int id = x * kThreadsPerGroup + tid;
+            return reinterpret_cast<uint4v*>(v_tile + L::v_at(id / kChunks, 16 * (id % kChunks)));
+        };
+        if (p.causal && diagonal) {
+            bool special = false;
+#pragma unroll
+            for (int x = 0; x < kChecks; ++x) special |= not_finite<kBf16>(*checked(x));
+            if (special) lds_special_tile = j + 1;
+        }
         tile_barrier();  // every wave finished reading K_j (and P.V of the previous tile)
         set_priority<0>();
+        const bool special = p.causal && diagonal && lds_special_tile == j + 1;
+        if (special) {
+#pragma unroll 1
+            for (int x = 0; x < kChecks; ++x) {
+                unsigned masks[3];
+                const uint4v clean = take_out_special<kBf16>(*checked(x), masks);
+                *checked(x) = clean;
+#pragma unroll
+                for (int kind = 0; kind < 3; ++kind)
+                    lds_special[kind][x * kThreadsPerGroup + tid] = static_cast<unsigned char>(masks[kind]);
+            }
+            __syncthreads();
+        }
         if (j + 1 < tiles) {
             issue_k(j + 1);
             issue_v(j + 1, v_buffer ^ 1);
@@ -414,63 +448,43 @@ __global__ __launch_bounds__(kThreadsPerGroup, 2) void packed_attention_kernel(c
         if (active) {
             uint4v ph[4];
             softmax_rows<kOB, kBf16>(st, s, c, ph);
-            const unsigned char* const v_tile = lds_v + (v_buffer ? L::kVBytes : 0);
             // V^T fragment of step t = (key step t / kOB, feature block t % kOB).
             auto v_frag = [&](int t) {
                 const unsigned char* const lo = v_tile + 16 * L::kVStride * (t / kOB) + v_lane[t % kOB];
                 return __builtin_bit_cast(uint4v, concat(read_tr16(lo), read_tr16(lo + 8 * L::kVStride)));
             };
             constexpr int kSteps = 4 * kOB;
-            bool special = false;
-            if (p.causal && masked) {
-                // A row's probability of a key that it does not see is 0, but 0 times an
-                // infinite or NaN value is NaN.
+            constexpr int kAhead = 3;
+            set_priority<0>();
+            uint4v vf[kAhead + 1];
 #pragma unroll
-                for (int t = 0; t < kSteps; ++t) special |= not_finite<kBf16>(v_frag(t));
-                special = __any(special);
+            for (int t = 0; t < kAhead; ++t)
+                if (t < kSteps) vf[t] = v_frag(t);
+#pragma unroll
+            for (int t = 0; t < kSteps; ++t) {
+                if (t + kAhead < kSteps) vf[(t + kAhead) % (kAhead + 1)] = v_frag(t + kAhead);
+                st.o[t % kOB] = mfma_32x32x16<kBf16>(vf[t % (kAhead + 1)], ph[t / kOB], st.o[t % kOB]);
+                __builtin_amdgcn_sched_barrier(0);
             }
-            if (!special) {
-                constexpr int kAhead = 3;
-                set_priority<0>();
-                uint4v vf[kAhead + 1];
-#pragma unroll
-                for (int t = 0; t < kAhead; ++t)
-                    if (t < kSteps) vf[t] = v_frag(t);
-#pragma unroll
-                for (int t = 0; t < kSteps; ++t) {
-                    if (t + kAhead < kSteps) vf[(t + kAhead) % (kAhead + 1)] = v_frag(t + kAhead);
-                    st.o[t % kOB] = mfma_32x32x16<kBf16>(vf[t % (kAhead + 1)], ph[t / kOB], st.o[t % kOB]);
-                    __builtin_amdgcn_sched_barrier(0);
-                }
-            } else {
-                // The finite values; then which of +inf, -inf and NaN the row sees, by how many.
-                constexpr std::uint32_t kOne = kBf16 ? 0x3f80u : 0x3c00u;
-                auto sees = [&](int ks) {
-                    uint4v out;
-#pragma unroll
-                    for (int e = 0; e < 8; e += 2) {
-                        const int key = 32 * (ks >> 1) + 8 * ((8 * (ks & 1) + e) >> 2) + (e & 3);
-                        out[e / 2] = (key <= seen ? kOne : 0u) | (key + 1 <= seen ? kOne << 16 : 0u);
-                    }
-                    return out;
-                };
-#pragma unroll
-                for (int fb = 0; fb < kOB; ++fb)
-#pragma unroll
-                    for (int ks = 0; ks < 4; ++ks)
-                        st.o[fb] = mfma_32x32x16<kBf16>(value_class<kBf16>(v_frag(ks * kOB + fb), 0), ph[ks], st.o[fb]);
+            if (special) {
 #pragma unroll 1
-                for (int kind = 1; kind < 4; ++kind) {
-                    const float value = kind == 1 ? INFINITY : kind == 2 ? -INFINITY : NAN;
+                for (int kind = 0; kind < 3; ++kind) {
+                    unsigned seen_bits[kChunks / 4] = {};  // features in which the row sees such a value
+#pragma unroll 1
+                    for (int key = 0; key < kTileKeys; ++key) {
+                        const auto* const bits = reinterpret_cast<const unsigned*>(lds_special[kind] + key * kChunks);
 #pragma unroll
-                    for (int fb = 0; fb < kOB; ++fb) {
-                        float16v count{};
-#pragma unroll
-                        for (int ks = 0; ks < 4; ++ks)
-                            count = mfma_32x32x16<kBf16>(value_class<kBf16>(v_frag(ks * kOB + fb), kind), sees(ks), count);
-#pragma unroll
-                        for (int e = 0; e < 16; ++e) st.o[fb][e] += count[e] > 0.0f ? value : 0.0f;
+                        for (int x = 0; x < kChunks / 4; ++x)
+                            if (key <= seen + 4 * h) seen_bits[x] |= bits[x];
                     }
+                    const float value = kind == 0 ? INFINITY : kind == 1 ? -INFINITY : NAN;
+#pragma unroll
+                    for (int fb = 0; fb < kOB; ++fb)
+#pragma unroll
+                        for (int e = 0; e < 16; ++e) {
+                            const int feature = (e < 8 ? 0 : kDP / 2 - 16) + 16 * fb + 8 * (e / 4) + e % 4;  // + 4 h
+                            st.o[fb][e] += (seen_bits[feature / 32] >> (feature % 32 + 4 * h)) & 1u ? value : 0.0f;
+                        }
                 }
             }
         }
@@ -483,19 +497,39 @@ __global__ __launch_bounds__(kThreadsPerGroup, 2) void packed_attention_kernel(c
     const float l = a + b;
     // 0: no key; NaN scores leave l NaN, and the row becomes NaN.
     const float inverse = l == 0.0f ? 0.0f : 1.0f / l;
-    if (tw + q < seq.q_len) {
-        std::uint16_t* const row = p.O + static_cast<std::int64_t>(seq.q0 + tw + q) * p.o_row + head * p.o_head;
+    // Rows leave through LDS as whole lines: stored from registers, an instruction writes 16
+    // bytes of each of 32 rows, and twice the bytes went to memory (16 x 1024 tokens, 32
+    // heads x 128: 262 MB for 134, 250 us; 227 so). The wave's region lies in the K
+    // tile or the V buffer that the last tile did not use: every wave has passed the last tile's
+    // second barrier, so none reads them. 16-byte chunk c of a row lies at chunk
+    // position (c + row) mod kChunks.
+    static_assert(L::kKBytes >= 2 * kRowsPerWave * kDP * 2 && L::kVBytes >= 2 * kRowsPerWave * kDP * 2, "two waves' rows fit a tile");
+    unsigned char* const region =
+        (wave < 2 ? lds_k : lds_v + (v_buffer ? L::kVBytes : 0)) + (wave & 1) * kRowsPerWave * kDP * 2;
+    auto chunk_at = [&](int row, int c) { return region + (row * kChunks + (c + row) % kChunks) * 16; };
 #pragma unroll
-        for (int fb = 0; fb < kOB; ++fb)
+    for (int fb = 0; fb < kOB; ++fb)
 #pragma unroll
-            for (int r4 = 0; r4 < 4; ++r4) {
-                const int feature = (r4 < 2 ? 0 : kDP / 2 - 16) + 16 * fb + 8 * r4 + 4 * h;
-                const float4v value{st.o[fb][4 * r4], st.o[fb][4 * r4 + 1], st.o[fb][4 * r4 + 2], st.o[fb][4 * r4 + 3]};
-                if (feature < d)
-                    *reinterpret_cast<uint2v*>(row + feature) =
-                        uint2v{pack_pair<kBf16>(value[0] * inverse, value[1] * inverse),
-                               pack_pair<kBf16>(value[2] * inverse, value[3] * inverse)};
-            }
+        for (int r4 = 0; r4 < 4; ++r4) {
+            const int feature = (r4 < 2 ? 0 : kDP / 2 - 16) + 16 * fb + 8 * r4;  // + 4 h
+            const float4v value{st.o[fb][4 * r4], st.o[fb][4 * r4 + 1], st.o[fb][4 * r4 + 2], st.o[fb][4 * r4 + 3]};
+            *reinterpret_cast<uint2v*>(chunk_at(q, feature / 8) + 8 * h) =
+                uint2v{pack_pair<kBf16>(value[0] * inverse, value[1] * inverse),
+                       pack_pair<kBf16>(value[2] * inverse, value[3] * inverse)};
+        }
+    std::uint16_t* const out = p.O + static_cast<std::int64_t>(seq.q0 + tw) * p.o_row + head * p.o_head;
+    constexpr int kStores = kRowsPerWave * kChunks / kWave;
+    uint4v piece[kStores];
+#pragma unroll
+    for (int x = 0; x < kStores; ++x) {
+        const int id = x * kWave + lane;
+        piece[x] = *reinterpret_cast<const uint4v*>(chunk_at(id / kChunks, id % kChunks));
+    }
+#pragma unroll
+    for (int x = 0; x < kStores; ++x) {
+        const int id = x * kWave + lane, row = id / kChunks, c = id % kChunks;
+        if (tw + row < seq.q_len && 8 * c < d)
+            __builtin_nontemporal_store(piece[x], reinterpret_cast<uint4v_dword*>(out + row * p.o_row + 8 * c));
     }
 }
 
