@@ -288,7 +288,13 @@ int tilemix_quantize_qk_strided(const uint16_t* Q, const uint16_t* K, int8_t* Q8
  * Keys and values that a row does not see do not reach it, whatever they hold.
  * Starts are clamped to 0 .. q_tokens / k_tokens; where they decrease, the
  * sequence is empty. q_tokens or batch 0: nothing to do. k_row_stride and
- * v_row_stride up to 2^24 elements (more: NotSupported). */
+ * v_row_stride up to 2^24 elements (more: NotSupported); more than 2^31 - 1
+ * blocks of 128 rows -> InvalidConfiguration.
+ * A call of few rows with many keys has its key ranges split over several
+ * workgroups, whose partial rows go to one of the split workspaces (see
+ * tilemix_attention) and are merged in order by the last of them: the same call
+ * gives the same bits. Under capture it uses none and is not split: slower, and
+ * rounded in another order. */
 typedef struct TileMixPackedAttentionArgs {
     const uint16_t* Q;
     const uint16_t* K;
@@ -419,7 +425,9 @@ int tilemix_cache4_gather(const TileMixCache4GatherArgs* args, void* stream);
  * any shape, one after the other (on one stream, or ordered by events; captured
  * calls that share one must not be replayed at once). Results do not depend on
  * what other calls left in it. Sums are taken in an order that lengths and
- * sizes decide: the same call gives the same bits. */
+ * sizes decide: the same call gives the same bits. Of
+ * at most T = max_pages * page_size tokens, batch * kv_heads * ceil(q_heads /
+ * kv_heads / 16) * (T / 32 + 8) past 2^29 -> InvalidConfiguration. */
 typedef struct TileMixCache4AttentionArgs {
     const uint16_t* Q;
     uint16_t* O;

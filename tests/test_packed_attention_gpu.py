@@ -279,3 +279,67 @@ def test_two_streams_at_once(tm, cuda):
     torch.cuda.synchronize()
     for o in outputs:
         _compare(o, expected, bound, "streams")
+
+
+# Few blocks of long walks: their key tiles are walked by several workgroups.
+SPLIT_CASES = [
+    _case([1], [1500], heads=(2, 1), d=128), _case([40], [1029], heads=(8, 2), d=128, dtype="bf16"),
+    _case([129, 64], [900, 1100], heads=(2, 2), d=64), _case([1, 0, 33, 0], [2000, 900, 1211, 3], heads=(4, 1), d=72, dtype="bf16"),
+    _case([300], [1700], heads=(3, 1), d=96), _case([70, 30], [1300, 1290], heads=(6, 3), d=128, causal=False),
+    _case([50, 20, 2000], [3000, 0, 40], heads=(1, 1), d=40), _case([1700], heads=(4, 2), d=128, dtype="bf16"),
+    _case([5, 6, 7, 8], [800, 900, 1000, 4000], heads=(16, 8), d=128), _case([64], [5000], heads=(1, 1), d=8, layout="wide"),
+    _case([40], [1500], heads=(4, 2), d=128, scale=3.0), _case([30], [1200], heads=(2, 1), d=64, scale=-0.3, layout="htd"),
+]
+
+
+@pytest.mark.parametrize("c", SPLIT_CASES, ids=_id)
+def test_split_calls_match_float64(tm, cuda, c):
+    p = _problem(c)
+    expected, bound = _expected(c, p)
+    o, again = _output(c, p), _output(c, p)
+    tm.check(tm.attention_packed(_args(tm, c, p, o)), "packed")
+    tm.check(tm.attention_packed(_args(tm, c, p, again)), "packed")
+    torch.cuda.synchronize()
+    _compare(o, expected, bound, _id(c))
+    assert torch.equal(o, again)  # parts are merged in their order, whichever is done first
+
+
+@pytest.mark.parametrize("what", [float("inf"), float("nan")])
+def test_split_rows_of_values_not_finite(tm, cuda, what):
+    """In the first range, in a diagonal tile of the last one, and behind what the first rows see."""
+    c = _case([40], [1200], heads=(4, 2), d=128, dtype="bf16")
+    p = _problem(c)
+    expected, bound = _expected(c, p)
+    q0, k0 = p["q_starts"][0], p["k_starts"][0]
+    for key, head, feature in ((10, 0, 3), (1165, 0, 70), (1199, 1, 127)):
+        p["v"][k0 + key, head, feature] = what
+        expected[q0 + max(key - 1160, 0):q0 + 40, 2 * head:2 * head + 2, feature] = what
+    o = _output(c, p)
+    tm.check(tm.attention_packed(_args(tm, c, p, o)))
+    torch.cuda.synchronize()
+    _compare(o, expected, bound, str(what))
+
+
+def test_split_calls_on_more_streams_than_workspaces_and_replayed(tm, cuda):
+    cases = [_case([40], [1500], heads=(4, 2), d=128, dtype="bf16"), _case([200, 10], [1100, 900], heads=(8, 2)),
+             _case([64], [3000], heads=(1, 1), d=128)]
+    problems = [_problem(c, 7 + i) for i, c in enumerate(cases)]
+    expected = [_expected(c, p) for c, p in zip(cases, problems)]
+    outputs = [_output(cases[i % 3], problems[i % 3]) for i in range(7)]
+    calls = [_args(tm, cases[i % 3], problems[i % 3], o) for i, o in enumerate(outputs)]
+    streams = [torch.cuda.Stream() for _ in range(6)]
+    graph = torch.cuda.CUDAGraph()
+    torch.cuda.synchronize()
+    with torch.cuda.graph(graph, stream=torch.cuda.Stream()):  # takes no workspace
+        tm.check(tm.attention_packed(calls[6]))
+    for turn in range(4):
+        for o in outputs:
+            o.fill_(GUARD)
+        torch.cuda.synchronize()
+        graph.replay()
+        for a, s in zip(calls, streams):
+            for _ in range(3):
+                tm.check(tm.attention_packed(a, stream=s))
+        torch.cuda.synchronize()
+        for i, o in enumerate(outputs):
+            _compare(o, *expected[i % 3], f"turn {turn} call {i}")

@@ -1706,10 +1706,11 @@ hipError_t launch_attention(AttnParams p, int units, bool precise, hipStream_t s
 // any stream had queued before its last one). Calls made while their stream is
 // being captured into a graph use none.
 static constexpr int kWorkspaces = 4;  // as many as hardware queues, HIP's default
-static constexpr std::size_t kSplitScratchFloats = std::size_t{8} << 20;  // 32 MiB each
-static constexpr std::size_t kSplitArrivals = 1024;
+using tilemix::kSplitArrivals;
+using tilemix::kSplitScratchFloats;
 static __device__ __align__(256) float split_scratch[kWorkspaces * kSplitScratchFloats];
 static __device__ unsigned split_arrivals[kWorkspaces * kSplitArrivals];  // zero between launches
+static __device__ __align__(256) float split_states[kWorkspaces * tilemix::kSplitStateFloats];  // call_with_workspace
 
 namespace tilemix {
 namespace {
@@ -1767,6 +1768,7 @@ struct Workspace {
 struct SplitDevice {
     float* scratch = nullptr;
     unsigned* arrivals = nullptr;
+    float* states = nullptr;
     Workspace workspaces[kWorkspaces];
     std::uint64_t calls = 0;
 };
@@ -1834,7 +1836,7 @@ int workspace_device(hipStream_t stream) {
     return device;
 }
 
-// Calls launch(scratch, arrivals), which enqueues kernels on `stream` that use
+// Calls launch(scratch, arrivals, states), which enqueues kernels on `stream` that use
 // one workspace of `device` (the current one), ordered after that workspace's
 // previous call and before its next one.
 template <typename Launch>
@@ -1844,7 +1846,7 @@ hipError_t with_workspace(int device, hipStream_t stream, Launch&& launch) {
     hipError_t status = hipSuccess;
     const int chosen = choose_workspace(state, stream);
     Workspace& workspace = state.workspaces[chosen];
-    if (!state.scratch || !state.arrivals || !workspace.done) {
+    if (!state.scratch || !state.arrivals || !state.states || !workspace.done) {
         // First split call on this device or workspace: another thread may be capturing a
         // graph in global mode, which would reject these runtime calls (they
         // enqueue no work), so this thread's capture mode is relaxed around
@@ -1861,6 +1863,10 @@ hipError_t with_workspace(int device, hipStream_t stream, Launch&& launch) {
             status = hipGetSymbolAddress(&address, HIP_SYMBOL(split_arrivals));
             if (status == hipSuccess) state.arrivals = static_cast<unsigned*>(address);
         }
+        if (status == hipSuccess && !state.states) {
+            status = hipGetSymbolAddress(&address, HIP_SYMBOL(split_states));
+            if (status == hipSuccess) state.states = static_cast<float*>(address);
+        }
         if (status == hipSuccess && !workspace.done)
             status = hipEventCreateWithFlags(&workspace.done, hipEventDisableTiming | hipEventDisableSystemFence);
         const hipError_t restored = hipThreadExchangeStreamCaptureMode(&mode);
@@ -1871,7 +1877,8 @@ hipError_t with_workspace(int device, hipStream_t stream, Launch&& launch) {
         status = hipStreamWaitEvent(stream, workspace.done, 0);
         if (status != hipSuccess) return status;
     }
-    status = launch(state.scratch + chosen * kSplitScratchFloats, state.arrivals + chosen * kSplitArrivals);
+    status = launch(state.scratch + chosen * kSplitScratchFloats, state.arrivals + chosen * kSplitArrivals,
+                    state.states + chosen * kSplitStateFloats);
     if (status != hipSuccess) return status;
     status = hipEventRecord(workspace.done, stream);
     if (status != hipSuccess) return status;
@@ -1880,6 +1887,19 @@ hipError_t with_workspace(int device, hipStream_t stream, Launch&& launch) {
     workspace.used = ++state.calls;
     return hipSuccess;
 }
+
+}  // namespace
+
+hipError_t call_with_workspace(hipStream_t stream, WorkspaceLaunch launch, void* context, bool& given) {
+    const int device = workspace_device(stream);
+    given = device >= 0;
+    if (!given) return hipSuccess;
+    return with_workspace(device, stream, [&](float* scratch, unsigned* arrivals, float* states) {
+        return launch(context, scratch, states, arrivals);
+    });
+}
+
+namespace {
 
 // launch_attention, with the key range split over several workgroups per
 // 128-row block when choose_split_tiles says so: the attention kernel writes
@@ -1896,7 +1916,7 @@ hipError_t launch_attention_split(AttnParams p, int units, bool precise, const S
     p.split_tiles = split_tiles;
     p.splits = (tiles + split_tiles - 1) / split_tiles;
     if (device < 0) return launch_attention(p, units, precise, stream);  // the ranges in turn
-    return with_workspace(device, stream, [&](float* scratch, unsigned*) {
+    return with_workspace(device, stream, [&](float* scratch, unsigned*, float*) {
         p.part_o = scratch;
         p.part_ml = scratch + static_cast<std::size_t>(p.heads) * p.splits * p.M * p.d;
         const hipError_t status = launch_attention(p, units, precise, stream);
@@ -1929,7 +1949,7 @@ hipError_t launch_decode_split(AttnParams p, int units, bool precise, hipStream_
     const int splits = plan_decode(p, units, kSplitScratchFloats, kSplitArrivals);
     const int device = splits > 1 ? workspace_device(stream) : -1;
     if (device < 0) return launch_decode(p, splits, precise, stream);  // the ranges in turn
-    return with_workspace(device, stream, [&](float* scratch, unsigned* arrivals) {
+    return with_workspace(device, stream, [&](float* scratch, unsigned* arrivals, float*) {
         p.part_o = scratch;
         p.arrivals = arrivals;
         return launch_decode(p, splits, precise, stream);

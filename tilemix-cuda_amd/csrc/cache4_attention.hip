@@ -134,18 +134,6 @@ __device__ __forceinline__ float over_16_lanes(float x, F&& f) {
     return f(x, step(std::integral_constant<int, 0x140>{}));
 }
 
-// Inclusive prefix sum over the lanes: DPP steps inside rows of 16 lanes, then the last
-// lane of each row added to the rows after it.
-__device__ __forceinline__ unsigned prefix_sum(unsigned x) {
-    int v = static_cast<int>(x);
-    v += __builtin_amdgcn_update_dpp(0, v, 0x111, 0xf, 0xf, false);  // row_shr 1, 2, 4, 8
-    v += __builtin_amdgcn_update_dpp(0, v, 0x112, 0xf, 0xf, false);
-    v += __builtin_amdgcn_update_dpp(0, v, 0x114, 0xf, 0xf, false);
-    v += __builtin_amdgcn_update_dpp(0, v, 0x118, 0xf, 0xf, false);
-    v += __builtin_amdgcn_update_dpp(0, v, 0x142, 0xa, 0xf, false);  // row_bcast 15 into rows 1 and 3
-    v += __builtin_amdgcn_update_dpp(0, v, 0x143, 0xc, 0xf, false);  // row_bcast 31 into rows 2 and 3
-    return static_cast<unsigned>(v);
-}
 __device__ __forceinline__ unsigned lane_value(unsigned v, int lane) {
     return static_cast<unsigned>(__builtin_amdgcn_readlane(static_cast<int>(v), lane));
 }

@@ -10,9 +10,10 @@
 //    K / V tile and end at the same diagonal, so a causal walk has less masked
 //    work than with 128 tokens of one head, and a short sequence fills its
 //    workgroup.
-//  * Which tokens a workgroup takes is found on the device (find_block), from the
+//  * Which tokens a workgroup takes is found on the device (find_work), from the
 //    lengths, blocks of more key tiles first: the host knows neither the lengths
 //    nor the longest.
+//  * Where the blocks are few, several workgroups walk a block's key tiles (kSplit).
 //  * Scores, softmax and P.V as in attention_kernel (attention.hip): S^T = K Q^T
 //    and O^T = V^T P^T on 32x32x16 MFMAs, probabilities kept in registers, K / V
 //    tiles by LDS DMA.
@@ -52,7 +53,18 @@ struct PackedParams {
     int causal;
     int negate;  // score_scale < 0: Q is negated
     float score_log2;  // |score_scale| log2(e)
+    // Of a split call: a workspace of the library.
+    float* part_o;
+    float* part_ml;
+    unsigned* arrivals;
 };
+
+constexpr int kMostParts = 512;  // workgroups of a split call
+constexpr int kLeastTiles = 4;   // key tiles of a split (8: 1 to 6 us more at 8 to 20 tiles a block)
+constexpr int kSplitWalk = 12;   // a split call's average walk, in key tiles
+static_assert(std::size_t{kMostParts} * kBlockRows * kMaxHeadDim <= kSplitScratchFloats &&
+                  std::size_t{kMostParts} * kBlockRows * 2 <= kSplitStateFloats && kMostParts <= kSplitArrivals,
+              "a split call's parts fit a workspace");
 
 // ------------------------------------------------------------ work items
 
@@ -98,16 +110,33 @@ __device__ __forceinline__ int blocks_walking(const Sequence& s, int shift, int 
     return blocks - (max(few, 0) >> shift);
 }
 
-// The sequence and block of work item `slot`, items of more key tiles first
-// (the last to start are the shortest; a long walk that starts last would run
-// alone); false past the last. Wave-uniform.
-__device__ __forceinline__ bool find_block(const PackedParams& p, int slot, int shift, int lane, Sequence& found, int& block) {
+// What a workgroup does: a block of a sequence, and of its key tiles one of `splits` ranges.
+struct Work {
+    Sequence seq;
+    int block;
+    int slot;  // the block's number among all
+    int split, splits;
+};
+
+// The work of place number `place` of a team, blocks of more key tiles first (the last
+// to start are the shortest; a long walk that starts last would run alone); false past
+// the last. kSplit: the team's `places` are dealt out to its blocks. Wave-uniform.
+template <bool kSplit>
+__device__ __forceinline__ bool find_work(const PackedParams& p, int place, int places, int shift, int lane, Work& work) {
     const bool causal = p.causal != 0;
+    auto divide = [&](int blocks) {
+        work.splits = kSplit ? max(places / max(blocks, 1), 1) : 1;
+        work.slot = kSplit ? place / work.splits : place;
+        work.split = kSplit ? place - work.slot * work.splits : 0;
+        return work.slot < blocks;
+    };
+    Sequence& found = work.seq;
     if (p.batch == 1) {
         found = sequence_at(p, 0);
         const int blocks = blocks_walking(found, shift, 0, causal);
-        block = blocks - 1 - slot;
-        return slot < blocks;
+        if (!divide(blocks)) return false;
+        work.block = blocks - 1 - work.slot;
+        return true;
     }
     Sequence mine{0, 0, 0, 0};
     if (lane < p.batch) mine = sequence_at(p, lane);
@@ -118,7 +147,8 @@ __device__ __forceinline__ bool find_block(const PackedParams& p, int slot, int 
             for (int b = lane + kWave; b < p.batch; b += kWave) n += blocks_walking(sequence_at(p, b), shift, tiles, causal);
         return wave_sum(n);
     };
-    if (count(0) <= slot) return false;
+    if (!divide(count(0))) return false;
+    const int slot = work.slot;
     // The most tiles of which more than `slot` blocks have as many.
     int low = 0, high = (p.k_tokens + kTileKeys - 1) / kTileKeys + 1;
     while (high - low > 1) {
@@ -135,12 +165,7 @@ __device__ __forceinline__ bool find_block(const PackedParams& p, int slot, int 
         if (b < p.batch) s = sequence_at(p, b);
         const int above = blocks_walking(s, shift, low + 1, causal);
         const int here = blocks_walking(s, shift, low, causal) - above;
-        int before = here;  // inclusive prefix over the lanes
-#pragma unroll
-        for (int step = 1; step < kWave; step <<= 1) {
-            const int other = __shfl_up(before, step);
-            if (lane >= step) before += other;
-        }
+        const int before = static_cast<int>(prefix_sum(here));
         const std::uint64_t past = __ballot(before > rest);
         if (past) {
             const int at = __builtin_ctzll(past);
@@ -150,7 +175,7 @@ __device__ __forceinline__ bool find_block(const PackedParams& p, int slot, int 
             found.k_len = __builtin_amdgcn_readlane(s.k_len, at);
             // Blocks of a sequence walk more tiles the later they are.
             const int blocks = blocks_walking(found, shift, 0, causal);
-            block = blocks - 1 - __builtin_amdgcn_readlane(above, at) - (rest - __builtin_amdgcn_readlane(before - here, at));
+            work.block = blocks - 1 - __builtin_amdgcn_readlane(above, at) - (rest - __builtin_amdgcn_readlane(before - here, at));
             return true;
         }
         rest -= __builtin_amdgcn_readlane(before, kWave - 1);
@@ -240,7 +265,9 @@ __device__ __forceinline__ uint4v take_out_special(uint4v v, unsigned (&masks)[3
     return v;
 }
 
-template <int DC, bool kBf16>
+// kSplit: few blocks, whose key tiles are walked by several workgroups each. Their rows
+// meet in the library's workspace, where the workgroup that arrives last merges them in order.
+template <int DC, bool kBf16, bool kSplit>
 __global__ __launch_bounds__(kThreadsPerGroup, 2) void packed_attention_kernel(const PackedParams p) {
     using L = Layout<DC>;
     constexpr int kDP = L::kDP;
@@ -271,16 +298,16 @@ __global__ __launch_bounds__(kThreadsPerGroup, 2) void packed_attention_kernel(c
     // Consecutive workgroups go to consecutive XCDs: with eight key heads (or a
     // multiple) each XCD keeps the K / V of its own heads in its L2.
     const int teams = p.kv_heads * p.chunks;
-    const int team = blockIdx.x % teams, slot = blockIdx.x / teams;
+    const int team = blockIdx.x % teams;
     const int kv_head = p.chunks == 1 ? team : team % p.kv_heads, chunk = p.chunks == 1 ? 0 : team / p.kv_heads;
     const int team_heads = 1 << p.team_shift;
     const int tokens = kBlockRows >> p.team_shift;
-    Sequence seq;
-    int block;
-    if (!find_block(p, slot, kBlockShift - p.team_shift, lane, seq, block)) return;
+    Work work;
+    if (!find_work<kSplit>(p, blockIdx.x / teams, gridDim.x / teams, kBlockShift - p.team_shift, lane, work)) return;
+    const Sequence& seq = work.seq;
     const int context = seq.k_len - seq.q_len;  // row i sees keys up to context + i
     const int head = kv_head * p.group + (chunk << p.team_shift) + (wave & (team_heads - 1));
-    const int t0 = block * tokens;
+    const int t0 = work.block * tokens;
     const int tw = t0 + kRowsPerWave * (wave >> p.team_shift);  // the wave's first token
 
     // ---------------------------------------------------------------- Q
@@ -361,7 +388,16 @@ __global__ __launch_bounds__(kThreadsPerGroup, 2) void packed_attention_kernel(c
     // Last key that some row of the workgroup / of the wave sees, and all rows of the wave see.
     const int rows_end = min(t0 + tokens, seq.q_len);
     const int group_last = p.causal ? min(context + rows_end, seq.k_len) - 1 : seq.k_len - 1;
-    const int tiles = group_last < 0 ? 0 : group_last / kTileKeys + 1;
+    const int all_tiles = group_last < 0 ? 0 : group_last / kTileKeys + 1;
+    // Ranges of at least kLeastTiles tiles (one, of none, of a block without keys). A tile takes
+    // 1.3 us, and the last workgroup merges a part in 0.8 us (latency of 64 KB): of n tiles,
+    // sqrt(1.6 n) ranges are soonest done (one token of 30000 keys, 8 key heads: 64 ranges 74 us,
+    // 27 54 us).
+    const int splits = kSplit ? min(work.splits, max(min(all_tiles / kLeastTiles, static_cast<int>(sqrtf(1.6f * all_tiles))), 1)) : 1;
+    if (kSplit && work.split >= splits) return;
+    auto range_start = [&](int split) { return split * (all_tiles / splits) + min(split, all_tiles % splits); };
+    const int first_tile = kSplit ? range_start(work.split) : 0;
+    const int tiles = kSplit ? range_start(work.split + 1) : all_tiles;
     const int wave_last = tw >= seq.q_len ? -1 : p.causal ? min(context + tw + kRowsPerWave, seq.k_len) - 1 : seq.k_len - 1;
     const int all_last = p.causal ? context + tw : seq.k_len - 1;
 
@@ -371,11 +407,11 @@ __global__ __launch_bounds__(kThreadsPerGroup, 2) void packed_attention_kernel(c
     const int first_hidden = p.causal ? context + t0 + 1 : seq.k_len;  // first key that some row of the workgroup does not see
     if (tid == 0) lds_special_tile = 0;
     int v_buffer = 0;
-    if (tiles > 0) {
-        issue_k(0);
-        issue_v(0, 0);
+    if (tiles > first_tile) {
+        issue_k(first_tile);
+        issue_v(first_tile, 0);
     }
-    for (int j = 0; j < tiles; ++j) {
+    for (int j = first_tile; j < tiles; ++j) {
         const int k0 = j * kTileKeys;
         tile_barrier();  // K_j, V_j landed; every wave finished P.V of the previous tile
         set_priority<2>();
@@ -494,7 +530,48 @@ __global__ __launch_bounds__(kThreadsPerGroup, 2) void packed_attention_kernel(c
     // ---------------------------------------------------------- epilogue
     float a = st.lsum, b = st.lsum;
     permlane32_swap(a, b);
-    const float l = a + b;
+    float l = a + b;
+    if constexpr (kSplit) {
+        if (splits > 1) {
+            // Parts: [item][split], O as the threads hold it, and (m, l) of the 128 rows.
+            constexpr int kQuads = 4 * kOB;
+            const int item = work.slot * teams + team, row = kRowsPerWave * wave + q;
+            const std::int64_t parts = gridDim.x;
+            const auto ro = shared_rows(p.part_o, parts * kQuads * kThreadsPerGroup * 4);
+            const auto rml = shared_rows(p.part_ml, parts * kBlockRows * 2);
+            auto o_at = [&](int part, int x) { return ((part * kQuads + x) * kThreadsPerGroup + tid) * 16; };
+            auto ml_at = [&](int part) { return (part * kBlockRows + row) * 8; };
+            const int first = item * work.splits;
+#pragma unroll
+            for (int x = 0; x < kQuads; ++x) {
+                const float16v& o = st.o[x / 4];
+                const int e = 4 * (x % 4);
+                __builtin_amdgcn_raw_buffer_store_b128(
+                    __builtin_bit_cast(uint4v, float4v{o[e], o[e + 1], o[e + 2], o[e + 3]}), ro, o_at(first + work.split, x), 0, kDeviceScope);
+            }
+            if (h == 0)
+                __builtin_amdgcn_raw_buffer_store_b64(__builtin_bit_cast(uint2v, float2v{st.m, l}), rml, ml_at(first + work.split), 0,
+                                                      kDeviceScope);
+            if (!last_arrival(p.arrivals + item, splits, &lds_special_tile)) return;
+            float m = -INFINITY;
+            l = 0.0f;
+#pragma unroll
+            for (int fb = 0; fb < kOB; ++fb) st.o[fb] = float16v{};
+#pragma unroll 1
+            for (int s = 0; s < splits; ++s) {
+                const float2v state = __builtin_bit_cast(float2v, __builtin_amdgcn_raw_buffer_load_b64(rml, ml_at(first + s), 0, kDeviceScope));
+                float4v part[kQuads];
+#pragma unroll
+                for (int x = 0; x < kQuads; ++x)
+                    part[x] = __builtin_bit_cast(float4v, __builtin_amdgcn_raw_buffer_load_b128(ro, o_at(first + s, x), 0, kDeviceScope));
+                const PartWeights w = merge_part(m, l, state[0], state[1]);
+#pragma unroll
+                for (int x = 0; x < kQuads; ++x)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) st.o[x / 4][4 * (x % 4) + e] = merged(st.o[x / 4][4 * (x % 4) + e], part[x][e], w);
+            }
+        }
+    }
     // 0: no key; NaN scores leave l NaN, and the row becomes NaN.
     const float inverse = l == 0.0f ? 0.0f : 1.0f / l;
     // Rows leave through LDS as whole lines: stored from registers, an instruction writes 16
@@ -533,13 +610,31 @@ __global__ __launch_bounds__(kThreadsPerGroup, 2) void packed_attention_kernel(c
     }
 }
 
-template <int DC>
+template <int DC, bool kSplit>
 void launch_packed(const PackedParams& p, bool bf16, unsigned grid, hipStream_t stream) {
     if (bf16)
-        packed_attention_kernel<DC, true><<<grid, kThreadsPerGroup, 0, stream>>>(p);
+        packed_attention_kernel<DC, true, kSplit><<<grid, kThreadsPerGroup, 0, stream>>>(p);
     else
-        packed_attention_kernel<DC, false><<<grid, kThreadsPerGroup, 0, stream>>>(p);
+        packed_attention_kernel<DC, false, kSplit><<<grid, kThreadsPerGroup, 0, stream>>>(p);
 }
+
+template <bool kSplit>
+hipError_t launch_packed(const PackedParams& p, bool bf16, unsigned grid, hipStream_t stream) {
+    switch ((p.d + 31) / 32) {
+        case 1: launch_packed<1, kSplit>(p, bf16, grid, stream); break;
+        case 2: launch_packed<2, kSplit>(p, bf16, grid, stream); break;
+        case 3: launch_packed<3, kSplit>(p, bf16, grid, stream); break;
+        default: launch_packed<4, kSplit>(p, bf16, grid, stream); break;
+    }
+    return hipGetLastError();
+}
+
+struct SplitCall {
+    PackedParams p;
+    bool bf16;
+    unsigned grid;
+    hipStream_t stream;
+};
 
 }  // namespace
 }  // namespace tilemix
@@ -592,15 +687,32 @@ extern "C" int tilemix_attention_packed(const TileMixPackedAttentionArgs* args, 
     const std::int64_t blocks = a.q_tokens / tokens + static_cast<std::int64_t>(std::min(a.batch, a.q_tokens));
     const std::int64_t grid = blocks * p.kv_heads * p.chunks;
     if (grid > 0x7fffffffLL) return hipErrorInvalidConfiguration;
-    const hipError_t found = check_device();
+    int units = 0;
+    const hipError_t found = check_device(&units);
     if (found != hipSuccess) return found;
     const bool bf16 = a.dtype == TILEMIX_DTYPE_BF16;
     const hipStream_t s = static_cast<hipStream_t>(stream);
-    switch ((a.d + 31) / 32) {
-        case 1: launch_packed<1>(p, bf16, static_cast<unsigned>(grid), s); break;
-        case 2: launch_packed<2>(p, bf16, static_cast<unsigned>(grid), s); break;
-        case 3: launch_packed<3>(p, bf16, static_cast<unsigned>(grid), s); break;
-        default: launch_packed<4>(p, bf16, static_cast<unsigned>(grid), s); break;
+    // Few blocks with long walks are split, into as many workgroups as are resident at
+    // once. The lengths are not known here, so the average walk decides (2 x 256 tokens, 16 heads
+    // x 128; in one piece and split): 6 tiles 17.7 and 19.8 us, 10 22.9 and 23.1, 18 33.6 and
+    // 26.0, 34 52 and 34, 122 154 and 58; 2 x 512 tokens after 7680 keys 168 and 85.
+    const std::int64_t teams = static_cast<std::int64_t>(p.kv_heads) * p.chunks, places = std::min(kMostParts, 2 * units) / teams;
+    const double rows = static_cast<double>(a.q_tokens) / a.batch, keys = static_cast<double>(a.k_tokens) / a.batch;
+    const double walk = (p.causal ? keys - 0.5 * std::min(rows, keys) : keys) / kTileKeys;
+    if (blocks <= places && 2 * ((rows + tokens - 1) / tokens) * a.batch <= static_cast<double>(places) && walk >= kSplitWalk) {
+        SplitCall call{p, bf16, static_cast<unsigned>(places * teams), s};
+        bool given = false;
+        const hipError_t status = call_with_workspace(
+            s,
+            [](void* context, float* scratch, float* states, unsigned* arrivals) {
+                SplitCall& c = *static_cast<SplitCall*>(context);
+                c.p.part_o = scratch;
+                c.p.part_ml = states;
+                c.p.arrivals = arrivals;
+                return launch_packed<true>(c.p, c.bf16, c.grid, c.stream);
+            },
+            &call, given);
+        if (given || status != hipSuccess) return status;
     }
-    return hipGetLastError();
+    return launch_packed<false>(p, bf16, static_cast<unsigned>(grid), s);
 }

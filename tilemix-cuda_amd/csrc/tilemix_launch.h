@@ -44,6 +44,17 @@ inline bool strided_heads_ok(int heads, int rows, int d, std::int64_t head_strid
 // otherwise), and its compute units.
 hipError_t check_device(int* compute_units = nullptr);
 
+// One of the library's split workspaces (attention.hip): floats of partial rows,
+// floats of their states, arrival counters that are zero between launches.
+inline constexpr std::size_t kSplitScratchFloats = std::size_t{8} << 20;  // 32 MiB
+inline constexpr std::size_t kSplitStateFloats = std::size_t{128} << 10;  // 512 KiB
+inline constexpr std::size_t kSplitArrivals = 1024;
+using WorkspaceLaunch = hipError_t (*)(void* context, float* scratch, float* states, unsigned* arrivals);
+// Calls launch(context, ...), which enqueues kernels on `stream` that use a workspace, ordered
+// before and after what else uses it. given: false, and nothing is called, where `stream` is
+// being captured (or the device has no workspace).
+hipError_t call_with_workspace(hipStream_t stream, WorkspaceLaunch launch, void* context, bool& given);
+
 QuantSide make_quant_side(const std::uint16_t* x, std::int8_t* x8, std::uint16_t* scales,
                           std::int64_t head_stride, int rows, int block_rows, std::int64_t row_stride);
 
