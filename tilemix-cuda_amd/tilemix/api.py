@@ -2,6 +2,7 @@
 from __future__ import annotations
 
 import ctypes
+import sys
 from dataclasses import dataclass
 from pathlib import Path
 from typing import Any, Optional
@@ -124,12 +125,11 @@ def _stream(stream: Any) -> Optional[int]:
     initialised the GPU no torch stream can be current: None is then the null
     stream."""
     if stream is None:
-        import sys
-
         torch = sys.modules.get("torch")
         if torch is None or not torch.cuda.is_initialized():
             return None
-        return torch.cuda.current_stream().cuda_stream or None
+        # As torch.cuda.current_stream().cuda_stream, without the Stream object: 0.5 us for 2.9.
+        return torch._C._cuda_getCurrentRawStream(torch.cuda.current_device()) or None
     if isinstance(stream, int):
         return stream or None
     return stream.cuda_stream or None
