@@ -288,8 +288,8 @@ int tilemix_quantize_qk_strided(const uint16_t* Q, const uint16_t* K, int8_t* Q8
  * Keys and values that a row does not see do not reach it, whatever they hold.
  * Starts are clamped to 0 .. q_tokens / k_tokens; where they decrease, the
  * sequence is empty. q_tokens or batch 0: nothing to do. k_row_stride and
- * v_row_stride up to 2^24 elements (more: NotSupported); more than 2^31 - 1
- * blocks of 128 rows -> InvalidConfiguration.
+ * v_row_stride up to 2^24 elements (more: NotSupported); 2^24 blocks of 128
+ * rows (tokens x heads) or more -> InvalidConfiguration.
  * A call of few rows with many keys has its key ranges split over several
  * workgroups, whose partial rows go to one of the split workspaces (see
  * tilemix_attention) and are merged in order by the last of them: the same call
@@ -349,13 +349,14 @@ size_t tilemix_cache4_bytes(int64_t pages, int page_size, int kv_heads, int d);
  * floats: rotary_dim / 2 cosines, then as many sines; rotary_dim 0: not read):
  * (y1, y2) = (x1 cos - x2 sin, x2 cos + x1 sin), fp32, each product rounded, of
  * the features i and i + rotary_dim / 2, or with `interleaved` 2 i and 2 i + 1.
- * Q (optional with Q_out; Q_out may be Q) -> Q_out, K -> K_out (optional; may be K)
- * rounded to dtype; the cache takes the keys before that rounding. V is cached as
+ * Q (optional with Q_out) -> Q_out, K -> K_out (optional) rounded to dtype, each
+ * possibly in place (with the same strides, else InvalidValue; no other overlap); the cache takes the keys before that rounding. V is cached as
  * it is. Token t goes to slots[t]; a slot outside the cache (a negative one, say,
  * for a padded row) caches nothing. A token whose position is outside the table is
  * passed over: neither cached nor rotated. Two tokens of one call must not have
  * the same slot: which bytes of which of them stay is not defined. tokens 0:
- * nothing to do. */
+ * nothing to do; about 2^28 or more (2^29 of d <= 64) -> InvalidConfiguration, as
+ * for tilemix_cache4_gather. */
 typedef struct TileMixCache4AppendArgs {
     const uint16_t* Q;
     const uint16_t* K;

@@ -481,6 +481,53 @@ def test_captured_step_takes_lengths_and_slots_at_replay(tm, cuda):
         assert torch.equal(eager, o)
 
 
+# Enough blocks that workgroups share sequences and have parts of two, with 8 and 16 rows
+# a workgroup, and one sequence in as many parts as there are.
+LARGE_DECODES = [
+    _decode([(37 * i * i) % 2500 for i in range(80)], heads=(8, 2), size=64), _decode([3000, 1, 0, 900, 2047], heads=(32, 2), d=128, size=128, dtype="bf16"),
+    _decode([9000], heads=(1, 1), d=128, size=32), _decode([1024] * 6, heads=(4, 4), d=72, size=64, dtype="bf16"),
+    _decode([300 + 7 * i for i in range(40)], heads=(20, 1), size=96, table_pad=2), _decode([31] * 300, heads=(2, 2), d=128),
+]
+
+
+def _run(tm, c, problem, workspace):
+    cache, table, _, pages = problem
+    o = torch.empty(len(c["lengths"]), c["heads"][0], c["d"], dtype=DT[c["dtype"]], device="cuda")
+    tm.check(tm.attention_cache4(_decode_args(tm, c, _queries(c).cuda(), o, cache, table, pages, workspace)))
+    torch.cuda.synchronize()
+    return o
+
+
+@pytest.mark.parametrize("c", LARGE_DECODES, ids=lambda c: f"{len(c['lengths'])}x{max(c['lengths'])}-h{c['heads'][0]}x{c['heads'][1]}-d{c['d']}-{c['dtype']}")
+def test_large_batches_match_float64(tm, cuda, workspace, c):
+    problem = _decode_problem(c)
+    expected, bound = _decode_expected(c, _queries(c), problem[0], problem[2])
+    _check(_run(tm, c, problem, workspace), expected, bound, "large")
+
+
+def test_a_workspace_serves_any_shape(tm, cuda):
+    """The same bits from one workspace after calls of other shapes as from a new one each."""
+    def new():
+        return torch.zeros(tm.attention_cache4_workspace_bytes(), dtype=torch.uint8, device="cuda")
+
+    one = new()
+    problems = [(c, _decode_problem(c)) for c in (LARGE_DECODES[3], DECODES[0], LARGE_DECODES[5], DECODES[11], LARGE_DECODES[4])]
+    for c, problem in problems + problems[::-1]:
+        assert torch.equal(_run(tm, c, problem, one), _run(tm, c, problem, new()))
+
+
+def test_queries_of_zeros_under_the_largest_scale(tm, cuda, workspace):
+    """Scores of 0 whatever the scale: the mean of the values."""
+    c = _decode([100, 33], heads=(4, 2), d=64, scale=3.4e38)
+    cache, table, slots, pages = _decode_problem(c)
+    q = torch.zeros_like(_queries(c))
+    expected, bound = _decode_expected(c, q, cache, slots)
+    o = torch.empty_like(q).cuda()
+    tm.check(tm.attention_cache4(_decode_args(tm, c, q.cuda(), o, cache, table, pages, workspace)))
+    torch.cuda.synchronize()
+    _check(o, expected, bound, "mean")
+
+
 def test_two_streams_with_their_own_workspaces(tm, cuda):
     c = _decode([4000, 900], heads=(4, 1), d=64, size=64)
     cache, table, slots, pages = _decode_problem(c)

@@ -343,3 +343,15 @@ def test_split_calls_on_more_streams_than_workspaces_and_replayed(tm, cuda):
         torch.cuda.synchronize()
         for i, o in enumerate(outputs):
             _compare(o, *expected[i % 3], f"turn {turn} call {i}")
+
+
+def test_queries_of_zeros_under_the_largest_scale(tm, cuda):
+    """Scores of 0 whatever the scale: the mean of the values."""
+    c = _case([70, 5], heads=(2, 1), scale=3.4e38)
+    p = _problem(c)
+    p["q"].zero_()
+    expected, bound = _expected({**c, "scale": 1.0}, p)
+    o = _output(c, p)
+    tm.check(tm.attention_packed(_args(tm, c, p, o)))
+    torch.cuda.synchronize()
+    _compare(o, expected, bound, "mean")

@@ -14,6 +14,7 @@ from tilemix import api, serving
 
 HEADER = Path(__file__).resolve().parent.parent / "include" / "tilemix_capi.h"
 INVALID, NOT_SUPPORTED = api.ERROR_INVALID_VALUE, api.ERROR_NOT_SUPPORTED
+CONFIGURATION = api.ERROR_INVALID_CONFIGURATION
 NAN, INF = float("nan"), float("inf")
 
 _memory = np.zeros(64, dtype=np.uint8)
@@ -124,6 +125,24 @@ def test_refusals_of_one_operator(tm):
     for stride in ("k_row_stride", "v_row_stride"):
         assert code("packed", **{stride: (1 << 24) + 8}) == NOT_SUPPORTED
     assert code("packed", q_tokens=-1) == INVALID and code("packed", k_tokens=-1) == INVALID
+
+
+def test_calls_too_large_for_a_launch(tm):
+    """Fewer than 2^32 threads and, for the decode step, 2^30 places of blocks."""
+    large = dict(kv_heads=1, d=128, tokens=1 << 28)
+    assert code("append", **large, q_heads=1) == CONFIGURATION and code("gather", **large) == CONFIGURATION
+    for tokens in (1 << 29, 2 ** 31 - 1):
+        assert code("append", **{**large, "d": 64, "tokens": tokens}, q_heads=1) == CONFIGURATION
+        assert code("gather", **{**large, "d": 64, "tokens": tokens}) == CONFIGURATION
+    assert code("packed", q_tokens=2 ** 31 - 1, q_heads=2) == CONFIGURATION
+    assert code("packed", q_tokens=1 << 27, q_heads=16, batch=1) == CONFIGURATION
+    assert code("decode", batch=1 << 20, max_pages=1 << 20) == CONFIGURATION
+    assert code("decode", batch=2 ** 31 - 1, max_pages=2 ** 31 - 1) == CONFIGURATION
+
+
+def test_rows_in_place_have_one_layout(tm):
+    for other in (dict(q_row_stride=512), dict(q_out_row_stride=512), dict(k_out_row_stride=256), dict(k_head_stride=128, k_row_stride=256)):
+        assert code("append", **other) == INVALID, other
 
 
 def test_calls_with_nothing_to_do(tm):

@@ -335,22 +335,20 @@ __global__ __launch_bounds__(kCacheThreads) void cache4_gather_kernel(const Gath
     rows_of(std::integral_constant<Kind, Kind::kValue>{}, p.v, max(first - keys, 0), last - keys);
 }
 
-// Heads that one wave takes in turn, and the grid: enough waves to fill the device.
-hipError_t plan_rows(int tokens, int tokens_per_wave, int heads, int& heads_per_wave, dim3& grid) {
-    constexpr int kWavesWanted = 4096;
-    const std::int64_t token_groups = (tokens - 1) / tokens_per_wave + 1;
+// Heads that one wave takes in turn, and the grid: enough waves to fill the device. Less than
+// 2^32 threads along a side, which is also what keeps token numbers in 32 bits.
+hipError_t plan_rows(int tokens, int groups, std::int64_t heads, int& heads_per_wave, dim3& grid) {
+    constexpr int kWavesWanted = 4096;  // (append and gather of 8192 tokens: 1024 62 us, 4096 58, 16384 67)
+    const std::int64_t token_groups = (tokens - 1) / (kWave / (8 * groups)) + 1;
     heads_per_wave = static_cast<int>(std::clamp<std::int64_t>(token_groups * heads / kWavesWanted, 1, heads));
-    const std::int64_t workgroups = (token_groups - 1) / kCacheWaves + 1;
-    grid = dim3(static_cast<unsigned>((workgroups + kXcds - 1) / kXcds * kXcds),
-                static_cast<unsigned>((heads - 1) / heads_per_wave + 1));
-    return grid.y > 65535 ? hipErrorInvalidConfiguration : hipSuccess;
+    const std::int64_t workgroups = ((token_groups - 1) / kCacheWaves + kXcds) / kXcds * kXcds;
+    if (workgroups > 0xffffffffLL / kCacheThreads) return hipErrorInvalidConfiguration;
+    grid = dim3(static_cast<unsigned>(workgroups), static_cast<unsigned>((heads - 1) / heads_per_wave + 1));  // y < 2 kWavesWanted
+    return hipSuccess;
 }
 
 template <int kGroups, Turn kTurn>
-hipError_t launch_append(AppendParams p, bool bf16, hipStream_t stream) {
-    dim3 grid;
-    const hipError_t planned = plan_rows(p.tokens, kWave / (8 * kGroups), p.q_heads + 2 * p.kv_heads, p.heads_per_wave, grid);
-    if (planned != hipSuccess) return planned;
+hipError_t launch_append(const AppendParams& p, dim3 grid, bool bf16, hipStream_t stream) {
     if (bf16)
         cache4_append_kernel<kGroups, true, kTurn><<<grid, kCacheThreads, 0, stream>>>(p);
     else
@@ -359,21 +357,22 @@ hipError_t launch_append(AppendParams p, bool bf16, hipStream_t stream) {
 }
 
 template <Turn kTurn>
-hipError_t launch_append(const AppendParams& p, bool bf16, hipStream_t stream) {
-    return p.cache.groups == 1 ? launch_append<1, kTurn>(p, bf16, stream) : launch_append<2, kTurn>(p, bf16, stream);
+hipError_t launch_append(const AppendParams& p, dim3 grid, bool bf16, hipStream_t stream) {
+    return p.cache.groups == 1 ? launch_append<1, kTurn>(p, grid, bf16, stream) : launch_append<2, kTurn>(p, grid, bf16, stream);
 }
 
 template <int kGroups>
-hipError_t launch_gather(GatherParams p, bool bf16, hipStream_t stream) {
-    dim3 grid;
-    const hipError_t planned =
-        plan_rows(p.tokens, kWave / (8 * kGroups), (p.k.out ? p.kv_heads : 0) + (p.v.out ? p.kv_heads : 0), p.heads_per_wave, grid);
-    if (planned != hipSuccess) return planned;
+hipError_t launch_gather(const GatherParams& p, dim3 grid, bool bf16, hipStream_t stream) {
     if (bf16)
         cache4_gather_kernel<kGroups, true><<<grid, kCacheThreads, 0, stream>>>(p);
     else
         cache4_gather_kernel<kGroups, false><<<grid, kCacheThreads, 0, stream>>>(p);
     return hipGetLastError();
+}
+
+// Rows written over what they are computed from have to be the same rows.
+bool in_place_ok(const TokenRows& rows) {
+    return rows.in != rows.out || (rows.in_rows.row == rows.out_rows.row && rows.in_rows.head == rows.out_rows.head);
 }
 
 bool dtype_ok(int dtype) { return dtype == TILEMIX_DTYPE_F16 || dtype == TILEMIX_DTYPE_BF16; }
@@ -416,7 +415,11 @@ extern "C" int tilemix_cache4_append(const TileMixCache4AppendArgs* args, void* 
         !make_rows(p.v.in_rows, a.V, a.tokens, a.kv_heads, a.d, a.v_row_stride, a.v_head_stride, 8))
         return hipErrorInvalidValue;
     if (a.tokens == 0) return hipSuccess;
-    if (!a.slots) return hipErrorInvalidValue;
+    if (!a.slots || (a.Q && !in_place_ok(p.q)) || !in_place_ok(p.k)) return hipErrorInvalidValue;
+    dim3 grid;
+    const hipError_t planned =
+        plan_rows(a.tokens, p.cache.groups, p.q_heads + std::int64_t{2} * a.kv_heads, p.heads_per_wave, grid);
+    if (planned != hipSuccess) return planned;
     p.cos_sin = a.cos_sin;
     p.token_positions = a.token_positions;
     p.slots = a.slots;
@@ -430,10 +433,10 @@ extern "C" int tilemix_cache4_append(const TileMixCache4AppendArgs* args, void* 
     if (found != hipSuccess) return found;
     const bool bf16 = a.dtype == TILEMIX_DTYPE_BF16;
     const hipStream_t s = static_cast<hipStream_t>(stream);
-    if (p.rotary == 0) return launch_append<Turn::kNone>(p, bf16, s);
-    if (a.interleaved) return launch_append<Turn::kPairs>(p, bf16, s);
+    if (p.rotary == 0) return launch_append<Turn::kNone>(p, grid, bf16, s);
+    if (a.interleaved) return launch_append<Turn::kPairs>(p, grid, bf16, s);
     const bool pieces = p.half % 8 == 0 && reinterpret_cast<std::uintptr_t>(p.cos_sin) % 16 == 0;
-    return pieces ? launch_append<Turn::kHalves>(p, bf16, s) : launch_append<Turn::kHalvesSingle>(p, bf16, s);
+    return pieces ? launch_append<Turn::kHalves>(p, grid, bf16, s) : launch_append<Turn::kHalvesSingle>(p, grid, bf16, s);
 }
 
 extern "C" int tilemix_cache4_gather(const TileMixCache4GatherArgs* args, void* stream) {
@@ -455,9 +458,13 @@ extern "C" int tilemix_cache4_gather(const TileMixCache4GatherArgs* args, void* 
     p.tokens = a.tokens;
     p.kv_heads = a.kv_heads;
     p.d = a.d;
+    dim3 grid;
+    const hipError_t planned =
+        plan_rows(a.tokens, p.cache.groups, std::int64_t{a.kv_heads} * ((a.K_out ? 1 : 0) + (a.V_out ? 1 : 0)), p.heads_per_wave, grid);
+    if (planned != hipSuccess) return planned;
     const hipError_t found = check_device();
     if (found != hipSuccess) return found;
     const bool bf16 = a.dtype == TILEMIX_DTYPE_BF16;
-    return p.cache.groups == 1 ? launch_gather<1>(p, bf16, static_cast<hipStream_t>(stream))
-                               : launch_gather<2>(p, bf16, static_cast<hipStream_t>(stream));
+    const hipStream_t s = static_cast<hipStream_t>(stream);
+    return p.cache.groups == 1 ? launch_gather<1>(p, grid, bf16, s) : launch_gather<2>(p, grid, bf16, s);
 }

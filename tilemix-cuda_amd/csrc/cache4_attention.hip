@@ -316,10 +316,13 @@ __global__ __launch_bounds__(kThreads, kGroupsPerUnit) void cache4_attention_ker
         // it would make every block wait for all of the blocks' loads.
         wait_vmcnt<0>();
     };
+    auto pages_of = [&](const Segment& s) __attribute__((always_inline)) {
+        return s.length == 0 ? 0 : static_cast<int>(static_cast<unsigned>(s.length - 1) / static_cast<unsigned>(p.cache.page_size)) + 1;
+    };
     auto enter = [&](const Segment& s) __attribute__((always_inline)) {
         table = p.table + s.sequence * p.table_stride;
         head_data = p.cache.data + head_of(s) * p.cache.head_bytes;
-        pages = (s.length + p.cache.page_size - 1) / p.cache.page_size;
+        pages = pages_of(s);
         end = s.end;
         step = s.first + wave;
         page = step / per_page;
@@ -376,7 +379,7 @@ __global__ __launch_bounds__(kThreads, kGroupsPerUnit) void cache4_attention_ker
     auto look_ahead = [&]() __attribute__((always_inline)) {
         has_next = after(segment, next);
         if (has_next) {
-            const int count = (next.length + p.cache.page_size - 1) / p.cache.page_size, first = wave / per_page;
+            const int count = pages_of(next), first = wave / per_page;
             next_page = first + lane < count ? p.table[next.sequence * p.table_stride + first + lane] : -1;
             load_queries(next_qf, next);
         }
@@ -800,8 +803,9 @@ extern "C" int tilemix_attention_cache4(const TileMixCache4AttentionArgs* args, 
     // A multiple of 32 under 2^31, so that block counts do not overflow.
     p.most_tokens = static_cast<int>(std::min<std::int64_t>(static_cast<std::int64_t>(a.max_pages) * a.page_size, 0x7fffffe0LL));
     p.negate = a.score_scale < 0.0f;
-    // (Of a score_scale of 0 the smallest number: a hidden token's -inf times it is still -inf.)
-    p.score_log2 = std::max(std::fabs(a.score_scale) * kLog2e, FLT_MIN);
+    // (Of a score_scale of 0 the smallest number: a hidden token's -inf times it is still -inf; of
+    // the largest a finite one, so that a score of 0 stays 0.)
+    p.score_log2 = std::clamp(std::fabs(a.score_scale) * kLog2e, FLT_MIN, FLT_MAX);
     const std::int64_t items = static_cast<std::int64_t>(a.batch) * a.kv_heads * p.tiles;
     // Places of one of them, and its end rounded up to a range's length.
     const std::int64_t most = 2 * ((p.most_tokens - 1) / kCacheKeys + 1 + kSwitch);

@@ -26,6 +26,7 @@
 #include "tilemix_capi.h"
 
 #include <algorithm>
+#include <cfloat>
 #include <cmath>
 
 namespace tilemix {
@@ -681,12 +682,12 @@ extern "C" int tilemix_attention_packed(const TileMixPackedAttentionArgs* args, 
     p.d = a.d;
     p.causal = a.causal != 0;
     p.negate = a.score_scale < 0.0f;
-    p.score_log2 = std::fabs(a.score_scale) * kLog2e;
+    p.score_log2 = std::min(std::fabs(a.score_scale) * kLog2e, FLT_MAX);  // finite: a score of 0 stays 0
     // Blocks of all sequences: each has at most one that is not full.
     const int tokens = kBlockRows >> p.team_shift;
     const std::int64_t blocks = a.q_tokens / tokens + static_cast<std::int64_t>(std::min(a.batch, a.q_tokens));
     const std::int64_t grid = blocks * p.kv_heads * p.chunks;
-    if (grid > 0x7fffffffLL) return hipErrorInvalidConfiguration;
+    if (grid > 0xffffffffLL / kThreadsPerGroup) return hipErrorInvalidConfiguration;  // threads of a launch
     int units = 0;
     const hipError_t found = check_device(&units);
     if (found != hipSuccess) return found;
