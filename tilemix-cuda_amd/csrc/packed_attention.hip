@@ -83,19 +83,20 @@ __device__ __forceinline__ Sequence sequence_at(const PackedParams& p, int b) {
     return s;
 }
 
-// Sum over the wave's lanes, in every lane (DPP steps as in wave_max_bits).
-__device__ __forceinline__ int wave_sum(int v) {
-    v += __builtin_amdgcn_update_dpp(0, v, 0xb1, 0xf, 0xf, false);
-    v += __builtin_amdgcn_update_dpp(0, v, 0x4e, 0xf, 0xf, false);
-    v += __builtin_amdgcn_update_dpp(0, v, 0x141, 0xf, 0xf, false);
-    v += __builtin_amdgcn_update_dpp(0, v, 0x140, 0xf, 0xf, false);
+// Sum or maximum over the wave's lanes, in every lane (DPP steps as in wave_max_bits).
+template <typename F>
+__device__ __forceinline__ int wave_reduce(int v, F f) {
+    v = f(v, __builtin_amdgcn_update_dpp(0, v, 0xb1, 0xf, 0xf, false));
+    v = f(v, __builtin_amdgcn_update_dpp(0, v, 0x4e, 0xf, 0xf, false));
+    v = f(v, __builtin_amdgcn_update_dpp(0, v, 0x141, 0xf, 0xf, false));
+    v = f(v, __builtin_amdgcn_update_dpp(0, v, 0x140, 0xf, 0xf, false));
     int a = v, b = v;
     asm volatile("s_nop 1\n\tv_permlane16_swap_b32 %0, %1" : "+v"(a), "+v"(b));
-    v = a + b;
+    v = f(a, b);
     a = v;
     b = v;
     asm volatile("s_nop 1\n\tv_permlane32_swap_b32 %0, %1" : "+v"(a), "+v"(b));
-    return __builtin_amdgcn_readfirstlane(a + b);
+    return __builtin_amdgcn_readfirstlane(f(a, b));
 }
 
 // Blocks of 1 << shift query tokens of a sequence that walk at least `tiles` key tiles.
@@ -146,12 +147,13 @@ __device__ __forceinline__ bool find_work(const PackedParams& p, int place, int 
         int n = blocks_walking(mine, shift, tiles, causal);
         if (!few)
             for (int b = lane + kWave; b < p.batch; b += kWave) n += blocks_walking(sequence_at(p, b), shift, tiles, causal);
-        return wave_sum(n);
+        return wave_reduce(n, [](int a, int b) { return a + b; });
     };
     if (!divide(count(0))) return false;
     const int slot = work.slot;
     // The most tiles of which more than `slot` blocks have as many.
-    int low = 0, high = (p.k_tokens + kTileKeys - 1) / kTileKeys + 1;
+    const unsigned keys = few ? wave_reduce(mine.k_len, [](int a, int b) { return max(a, b); }) : p.k_tokens;
+    int low = 0, high = static_cast<int>((keys + kTileKeys - 1) / kTileKeys) + 1;
     while (high - low > 1) {
         const int middle = (low + high) >> 1;
         if (count(middle) > slot)
@@ -160,10 +162,10 @@ __device__ __forceinline__ bool find_work(const PackedParams& p, int place, int 
             high = middle;
     }
     int rest = slot - count(low + 1);  // among the blocks of exactly `low` tiles
-    for (int base = 0;; base += kWave) {
+    for (int base = 0; base < p.batch; base += kWave) {
         const int b = base + lane;
-        Sequence s{0, 0, 0, 0};
-        if (b < p.batch) s = sequence_at(p, b);
+        Sequence s = mine;
+        if (base) s = b < p.batch ? sequence_at(p, b) : Sequence{0, 0, 0, 0};
         const int above = blocks_walking(s, shift, low + 1, causal);
         const int here = blocks_walking(s, shift, low, causal) - above;
         const int before = static_cast<int>(prefix_sum(here));
@@ -181,6 +183,7 @@ __device__ __forceinline__ bool find_work(const PackedParams& p, int place, int 
         }
         rest -= __builtin_amdgcn_readlane(before, kWave - 1);
     }
+    return false;  // (the starts changed meanwhile)
 }
 
 // ------------------------------------------------------- 16-bit arithmetic
