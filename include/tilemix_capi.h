@@ -293,8 +293,9 @@ int tilemix_quantize_qk_strided(const uint16_t* Q, const uint16_t* K, int8_t* Q8
  * A call of few rows with many keys has its key ranges split over several
  * workgroups, whose partial rows go to one of the split workspaces (see
  * tilemix_attention) and are merged in order by the last of them: the same call
- * gives the same bits. Under capture it uses none and is not split: slower, and
- * rounded in another order. */
+ * gives the same bits. Under capture it uses none: one workgroup takes a block's
+ * ranges in turn and merges them in the same order, for the eager call's bits at
+ * an unsplit call's speed. */
 typedef struct TileMixPackedAttentionArgs {
     const uint16_t* Q;
     const uint16_t* K;

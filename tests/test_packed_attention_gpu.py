@@ -330,7 +330,7 @@ def test_split_calls_on_more_streams_than_workspaces_and_replayed(tm, cuda):
     streams = [torch.cuda.Stream() for _ in range(6)]
     graph = torch.cuda.CUDAGraph()
     torch.cuda.synchronize()
-    with torch.cuda.graph(graph, stream=torch.cuda.Stream()):  # takes no workspace
+    with torch.cuda.graph(graph, stream=torch.cuda.Stream()):  # takes no workspace, and the same ranges in turn
         tm.check(tm.attention_packed(calls[6]))
     for turn in range(4):
         for o in outputs:
@@ -355,3 +355,40 @@ def test_queries_of_zeros_under_the_largest_scale(tm, cuda):
     tm.check(tm.attention_packed(_args(tm, c, p, o)))
     torch.cuda.synchronize()
     _compare(o, expected, bound, "mean")
+
+
+@pytest.mark.parametrize("c", SPLIT_CASES, ids=_id)
+def test_split_calls_replay_with_the_same_bits(tm, cuda, c):
+    """A captured call has no workspace: one workgroup takes a block's ranges in turn."""
+    p = _problem(c)
+    eager, o = _output(c, p), _output(c, p)
+    tm.check(tm.attention_packed(_args(tm, c, p, eager)), "packed")
+    args = _args(tm, c, p, o)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=torch.cuda.Stream()):
+        tm.check(tm.attention_packed(args))
+    for turn in range(3):
+        o.fill_(GUARD)
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(o.nan_to_num(nan=77.0), eager.nan_to_num(nan=77.0)), turn
+        eager.mul_(1)  # work of its own between the replays
+
+
+def test_replays_keep_values_not_finite(tm, cuda):
+    c = _case([40], [1200], heads=(4, 2), d=128)
+    p = _problem(c)
+    for key, what in ((10, math.inf), (1170, math.nan), (1190, -math.inf), (1199, math.inf)):
+        p["v"][p["k_starts"][0] + key, 0, key % 128] = what
+    eager, o = _output(c, p), _output(c, p)
+    tm.check(tm.attention_packed(_args(tm, c, p, eager)))
+    args = _args(tm, c, p, o)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=torch.cuda.Stream()):
+        tm.check(tm.attention_packed(args))
+    for _ in range(3):
+        o.fill_(GUARD)
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(o.nan_to_num(nan=77.0), eager.nan_to_num(nan=77.0))
+    assert torch.isinf(eager[:, :2]).any() and torch.isnan(eager[:, :2]).any() and torch.isfinite(eager[p["q_starts"][0]:p["q_starts"][1], 2:]).all()

@@ -54,6 +54,7 @@ struct PackedParams {
     int causal;
     int negate;  // score_scale < 0: Q is negated
     float score_log2;  // |score_scale| log2(e)
+    int places;        // workgroups of a team that share its blocks' key tiles; 0: one each
     // Of a split call: a workspace of the library.
     float* part_o;
     float* part_ml;
@@ -117,17 +118,17 @@ struct Work {
     Sequence seq;
     int block;
     int slot;  // the block's number among all
-    int split, splits;
+    int split, splits;  // at most `splits` ranges of its key tiles; kSplit: which of them
 };
 
 // The work of place number `place` of a team, blocks of more key tiles first (the last
 // to start are the shortest; a long walk that starts last would run alone); false past
 // the last. kSplit: the team's `places` are dealt out to its blocks. Wave-uniform.
 template <bool kSplit>
-__device__ __forceinline__ bool find_work(const PackedParams& p, int place, int places, int shift, int lane, Work& work) {
+__device__ __forceinline__ bool find_work(const PackedParams& p, int place, int shift, int lane, Work& work) {
     const bool causal = p.causal != 0;
     auto divide = [&](int blocks) {
-        work.splits = kSplit ? max(places / max(blocks, 1), 1) : 1;
+        work.splits = max(p.places / max(blocks, 1), 1);
         work.slot = kSplit ? place / work.splits : place;
         work.split = kSplit ? place - work.slot * work.splits : 0;
         return work.slot < blocks;
@@ -269,10 +270,15 @@ __device__ __forceinline__ uint4v take_out_special(uint4v v, unsigned (&masks)[3
     return v;
 }
 
-// kSplit: few blocks, whose key tiles are walked by several workgroups each. Their rows
-// meet in the library's workspace, where the workgroup that arrives last merges them in order.
-template <int DC, bool kBf16, bool kSplit>
+// How a block's key tiles are walked: in one piece; in ranges, each by a workgroup of its own,
+// whose rows meet in the library's workspace, where the workgroup that arrives last
+// merges them in order; in the same ranges by one workgroup, which merges them in the same order
+// for the same bits (captured calls, which have no workspace).
+enum class Walk { kWhole, kSplit, kInTurn };
+
+template <int DC, bool kBf16, Walk kWalk>
 __global__ __launch_bounds__(kThreadsPerGroup, 2) void packed_attention_kernel(const PackedParams p) {
+    constexpr bool kSplit = kWalk == Walk::kSplit, kInTurn = kWalk == Walk::kInTurn;
     using L = Layout<DC>;
     constexpr int kDP = L::kDP;
     constexpr int kOB = DC;
@@ -285,6 +291,11 @@ __global__ __launch_bounds__(kThreadsPerGroup, 2) void packed_attention_kernel(c
     constexpr int kChunks = kDP / 8;
     __shared__ __attribute__((aligned(16))) unsigned char lds_special[3][kTileKeys * kChunks];
     __shared__ int lds_special_tile;
+    constexpr int kQuads = 4 * kOB;
+    // kInTurn: O of the ranges so far, [quad][thread]. (Dynamic, as an array of known size would
+    // have the compiler allocate accumulation registers for one workgroup a CU, which the softmax
+    // pays for: 2 x 512 tokens after 7680 keys 245 us, 195 so; 168 in one piece.)
+    extern __shared__ float4v lds_merged[];
     unsigned char* const lds_k = smem;
     unsigned char* const lds_v = smem + L::kKBytes;
     const unsigned lds_k_address = lds_address_of(smem);
@@ -307,7 +318,7 @@ __global__ __launch_bounds__(kThreadsPerGroup, 2) void packed_attention_kernel(c
     const int team_heads = 1 << p.team_shift;
     const int tokens = kBlockRows >> p.team_shift;
     Work work;
-    if (!find_work<kSplit>(p, blockIdx.x / teams, gridDim.x / teams, kBlockShift - p.team_shift, lane, work)) return;
+    if (!find_work<kSplit>(p, blockIdx.x / teams, kBlockShift - p.team_shift, lane, work)) return;
     const Sequence& seq = work.seq;
     const int context = seq.k_len - seq.q_len;  // row i sees keys up to context + i
     const int head = kv_head * p.group + (chunk << p.team_shift) + (wave & (team_heads - 1));
@@ -397,7 +408,8 @@ __global__ __launch_bounds__(kThreadsPerGroup, 2) void packed_attention_kernel(c
     // 1.3 us, and the last workgroup merges a part in 0.8 us (latency of 64 KB): of n tiles,
     // sqrt(1.6 n) ranges are soonest done (one token of 30000 keys, 8 key heads: 64 ranges 74 us,
     // 27 54 us).
-    const int splits = kSplit ? min(work.splits, max(min(all_tiles / kLeastTiles, static_cast<int>(sqrtf(1.6f * all_tiles))), 1)) : 1;
+    const int splits =
+        kWalk == Walk::kWhole ? 1 : min(work.splits, max(min(all_tiles / kLeastTiles, static_cast<int>(sqrtf(1.6f * all_tiles))), 1));
     if (kSplit && work.split >= splits) return;
     auto range_start = [&](int split) { return split * (all_tiles / splits) + min(split, all_tiles % splits); };
     const int first_tile = kSplit ? range_start(work.split) : 0;
@@ -411,6 +423,14 @@ __global__ __launch_bounds__(kThreadsPerGroup, 2) void packed_attention_kernel(c
     const int first_hidden = p.causal ? context + t0 + 1 : seq.k_len;  // first key that some row of the workgroup does not see
     if (tid == 0) lds_special_tile = 0;
     int v_buffer = 0;
+    // kInTurn: the range under way, and the merged rows' states.
+    int range = 0, range_end = range_start(1);
+    float merged_m = -INFINITY, merged_l = 0.0f;
+    auto row_sum = [&]() __attribute__((always_inline)) {
+        float a = st.lsum, b = st.lsum;
+        permlane32_swap(a, b);
+        return a + b;
+    };
     if (tiles > first_tile) {
         issue_k(first_tile);
         issue_v(first_tile, 0);
@@ -529,16 +549,39 @@ __global__ __launch_bounds__(kThreadsPerGroup, 2) void packed_attention_kernel(c
             }
         }
         v_buffer ^= 1;
+        if (kInTurn && splits > 1 && j + 1 == range_end) {
+            const PartWeights w = merge_part(merged_m, merged_l, st.m, row_sum());
+#pragma unroll
+            for (int x = 0; x < kQuads; ++x) {
+                float4v& all = lds_merged[x * kThreadsPerGroup + tid];
+                const float16v& o = st.o[x / 4];
+                const int e = 4 * (x % 4);
+                all = merged(range == 0 ? float4v{0.0f, 0.0f, 0.0f, 0.0f} : all, float4v{o[e], o[e + 1], o[e + 2], o[e + 3]}, w);
+            }
+#pragma unroll
+            for (int fb = 0; fb < kOB; ++fb) st.o[fb] = float16v{};
+            st.lsum = 0.0f;
+            st.m = -INFINITY;
+            range_end = range_start(++range + 1);
+        }
     }
 
     // ---------------------------------------------------------- epilogue
-    float a = st.lsum, b = st.lsum;
-    permlane32_swap(a, b);
-    float l = a + b;
+    float l = row_sum();
+    if constexpr (kInTurn) {
+        if (splits > 1) {
+            l = merged_l;
+#pragma unroll
+            for (int x = 0; x < kQuads; ++x) {
+                const float4v all = lds_merged[x * kThreadsPerGroup + tid];
+#pragma unroll
+                for (int e = 0; e < 4; ++e) st.o[x / 4][4 * (x % 4) + e] = all[e];
+            }
+        }
+    }
     if constexpr (kSplit) {
         if (splits > 1) {
             // Parts: [item][split], O as the threads hold it, and (m, l) of the 128 rows.
-            constexpr int kQuads = 4 * kOB;
             const int item = work.slot * teams + team, row = kRowsPerWave * wave + q;
             const std::int64_t parts = gridDim.x;
             const auto ro = shared_rows(p.part_o, parts * kQuads * kThreadsPerGroup * 4);
@@ -614,21 +657,23 @@ __global__ __launch_bounds__(kThreadsPerGroup, 2) void packed_attention_kernel(c
     }
 }
 
-template <int DC, bool kSplit>
+template <int DC, Walk kWalk>
 void launch_packed(const PackedParams& p, bool bf16, unsigned grid, hipStream_t stream) {
+    constexpr std::size_t kMerged = kWalk == Walk::kInTurn ? std::size_t{kBlockRows} * 32 * DC * sizeof(float) : 0;
     if (bf16)
-        packed_attention_kernel<DC, true, kSplit><<<grid, kThreadsPerGroup, 0, stream>>>(p);
+        packed_attention_kernel<DC, true, kWalk><<<grid, kThreadsPerGroup, kMerged, stream>>>(p);
     else
-        packed_attention_kernel<DC, false, kSplit><<<grid, kThreadsPerGroup, 0, stream>>>(p);
+        packed_attention_kernel<DC, false, kWalk><<<grid, kThreadsPerGroup, kMerged, stream>>>(p);
 }
 
-template <bool kSplit>
-hipError_t launch_packed(const PackedParams& p, bool bf16, unsigned grid, hipStream_t stream) {
+template <Walk kWalk>
+hipError_t launch_packed(const PackedParams& p, bool bf16, std::int64_t workgroups, hipStream_t stream) {
+    const unsigned grid = static_cast<unsigned>(workgroups);
     switch ((p.d + 31) / 32) {
-        case 1: launch_packed<1, kSplit>(p, bf16, grid, stream); break;
-        case 2: launch_packed<2, kSplit>(p, bf16, grid, stream); break;
-        case 3: launch_packed<3, kSplit>(p, bf16, grid, stream); break;
-        default: launch_packed<4, kSplit>(p, bf16, grid, stream); break;
+        case 1: launch_packed<1, kWalk>(p, bf16, grid, stream); break;
+        case 2: launch_packed<2, kWalk>(p, bf16, grid, stream); break;
+        case 3: launch_packed<3, kWalk>(p, bf16, grid, stream); break;
+        default: launch_packed<4, kWalk>(p, bf16, grid, stream); break;
     }
     return hipGetLastError();
 }
@@ -636,7 +681,7 @@ hipError_t launch_packed(const PackedParams& p, bool bf16, unsigned grid, hipStr
 struct SplitCall {
     PackedParams p;
     bool bf16;
-    unsigned grid;
+    std::int64_t grid;
     hipStream_t stream;
 };
 
@@ -704,7 +749,8 @@ extern "C" int tilemix_attention_packed(const TileMixPackedAttentionArgs* args, 
     const double rows = static_cast<double>(a.q_tokens) / a.batch, keys = static_cast<double>(a.k_tokens) / a.batch;
     const double walk = (p.causal ? keys - 0.5 * std::min(rows, keys) : keys) / kTileKeys;
     if (blocks <= places && 2 * ((rows + tokens - 1) / tokens) * a.batch <= static_cast<double>(places) && walk >= kSplitWalk) {
-        SplitCall call{p, bf16, static_cast<unsigned>(places * teams), s};
+        p.places = static_cast<int>(places);
+        SplitCall call{p, bf16, places * teams, s};
         bool given = false;
         const hipError_t status = call_with_workspace(
             s,
@@ -713,10 +759,11 @@ extern "C" int tilemix_attention_packed(const TileMixPackedAttentionArgs* args, 
                 c.p.part_o = scratch;
                 c.p.part_ml = states;
                 c.p.arrivals = arrivals;
-                return launch_packed<true>(c.p, c.bf16, c.grid, c.stream);
+                return launch_packed<Walk::kSplit>(c.p, c.bf16, c.grid, c.stream);
             },
             &call, given);
         if (given || status != hipSuccess) return status;
+        return launch_packed<Walk::kInTurn>(p, bf16, grid, s);
     }
-    return launch_packed<false>(p, bf16, static_cast<unsigned>(grid), s);
+    return launch_packed<Walk::kWhole>(p, bf16, grid, s);
 }
