@@ -436,6 +436,7 @@ def attention_kernel_name(w, precise: bool) -> str:
 
 # Sources whose change invalidates a recorded traffic measurement.
 STAMPED_SOURCES = ["tilemix-cuda_amd/csrc/attention.hip", "tilemix-cuda_amd/csrc/attention_common.h",
+                   "tilemix-cuda_amd/csrc/attention_tiles.h",
                    "tilemix-cuda_amd/csrc/attention_rules.h",
                    "tilemix-cuda_amd/csrc/tilemix_device.h", "tilemix-cuda_amd/csrc/tilemix_launch.h",
                    "tilemix-cuda_amd/csrc/quantize.hip", "tilemix-cuda_amd/build.py"]
