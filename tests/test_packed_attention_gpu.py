@@ -392,3 +392,40 @@ def test_replays_keep_values_not_finite(tm, cuda):
         torch.cuda.synchronize()
         assert torch.equal(o.nan_to_num(nan=77.0), eager.nan_to_num(nan=77.0))
     assert torch.isinf(eager[:, :2]).any() and torch.isnan(eager[:, :2]).any() and torch.isfinite(eager[p["q_starts"][0]:p["q_starts"][1], 2:]).all()
+
+
+# More sequences than a wave has lanes are found by their starts.
+MANY = [
+    _case([(3 * i) % 5 for i in range(1000)], heads=(2, 1)), _case([0] * 200 + [130, 0, 1] + [0] * 90, heads=(4, 2), dtype="bf16"),
+    _case([33] * 65, heads=(1, 1), d=128, pad=(700, 300)), _case([1] * 129, [(17 * i) % 90 for i in range(129)], heads=(8, 2), d=128),
+    _case([64] * 70, heads=(3, 3), d=40, causal=False), _case([200] + [1] * 80 + [300], heads=(4, 4), dtype="bf16"),
+    # Split: few rows each, many keys.
+    _case([1 + i % 3 for i in range(70)], [700 + 11 * i for i in range(70)], heads=(1, 1)),
+    _case([0, 40] * 40, [0, 1500] * 40, heads=(2, 1), dtype="bf16"),
+]
+
+
+@pytest.mark.parametrize("c", MANY, ids=_id)
+def test_many_sequences(tm, cuda, c):
+    p = _problem(c)
+    expected, bound = _expected(c, p)
+    o = _output(c, p)
+    tm.check(tm.attention_packed(_args(tm, c, p, o)), "packed")
+    torch.cuda.synchronize()
+    _compare(o, expected, bound, _id(c))
+
+
+def test_many_starts_that_make_no_sense_stay_inside(tm, cuda):
+    """Rows outside the tensor are neither read nor written, whatever the starts hold."""
+    c = _case([4] * 100, heads=(4, 2), d=64)
+    p = _problem(c)
+    gen = torch.Generator().manual_seed(5)
+    o = _output(c, p)
+    whole = torch.full((o.numel() + 2 * 4096,), GUARD, dtype=o.dtype, device="cuda")
+    inside = whole[4096:-4096].view(o.shape)
+    for _ in range(4):
+        starts = torch.randint(-2 ** 31, 2 ** 31 - 1, (101,), generator=gen).to(torch.int32)
+        starts[::3] = torch.randint(0, p["q"].shape[0], (34,), generator=gen).to(torch.int32)
+        tm.check(tm.attention_packed(_args(tm, c, p, inside, q_starts=starts.cuda(), k_starts=starts.flip(0).cuda())))
+        torch.cuda.synchronize()
+    assert (whole[:4096] == GUARD).all() and (whole[-4096:] == GUARD).all()

@@ -127,12 +127,17 @@ struct Work {
     int split, splits;  // at most `splits` ranges of its key tiles; kSplit: which of them
 };
 
-// The work of place number `place` of a team, blocks of more key tiles first (the last
-// to start are the shortest; a long walk that starts last would run alone); false past
-// the last. kSplit: the team's `places` are dealt out to its blocks. Wave-uniform.
+// The work of place number `place` of a team, false past the last. kSplit: the team's
+// `places` are dealt out to its blocks. Wave-uniform.
+//
+// Up to 64 sequences, one a lane: blocks of more key tiles first (the last to start are the
+// shortest; a long walk that starts last would run alone), found by a search over tile
+// counts. More sequences keep their order, as every step of that search would read all of
+// their lengths (1000 sequences of 50 tokens, 32 heads: 707 us, 150 so): sequence b's blocks
+// have the numbers from floor(start / tokens of a block) + b on, which leaves room for
+// all of them, and is found by a search over the starts. Numbers left over have no work.
 template <bool kSplit>
 __device__ __forceinline__ bool find_work(const PackedParams& p, int place, int shift, int lane, Work& work) {
-    const bool causal = p.causal != 0;
     auto divide = [&](int blocks) {
         work.splits = max(p.places / max(blocks, 1), 1);
         work.slot = kSplit ? place / work.splits : place;
@@ -142,55 +147,57 @@ __device__ __forceinline__ bool find_work(const PackedParams& p, int place, int 
     Sequence& found = work.seq;
     if (p.batch == 1) {
         found = sequence_at(p, 0);
-        const int blocks = blocks_walking(found, shift, 0, causal);
+        const int blocks = blocks_walking(found, shift, 0, false);
         if (!divide(blocks)) return false;
         work.block = blocks - 1 - work.slot;
         return true;
     }
+    if (p.batch > kWave) {
+        auto number_of = [&](int b) { return (min(max(p.q_starts[b], 0), p.q_tokens) >> shift) + b; };
+        if (!divide(number_of(p.batch))) return false;
+        int low = 0, count = p.batch;  // the last of these whose number is at most the slot
+        for (int step = count; step > 1;) {
+            step = (count + kWave - 1) / kWave;
+            const bool reached = lane * step < count && number_of(low + lane * step) <= work.slot;
+            const std::uint64_t those = __ballot(reached);
+            if (!those) return false;  // rows before the first sequence
+            const int last = (kWave - 1 - __builtin_clzll(those)) * step;
+            low += last;
+            count = min(count - last, step);
+        }
+        low = __builtin_amdgcn_readfirstlane(low);
+        found = sequence_at(p, low);
+        work.block = blocks_walking(found, shift, 0, false) - 1 - (work.slot - number_of(low));
+        return work.block >= 0;
+    }
+    const bool causal = p.causal != 0;
     Sequence mine{0, 0, 0, 0};
     if (lane < p.batch) mine = sequence_at(p, lane);
-    const bool few = p.batch <= kWave;
-    auto count = [&](int tiles) {
-        int n = blocks_walking(mine, shift, tiles, causal);
-        if (!few)
-            for (int b = lane + kWave; b < p.batch; b += kWave) n += blocks_walking(sequence_at(p, b), shift, tiles, causal);
-        return wave_reduce(n, [](int a, int b) { return a + b; });
-    };
+    auto count = [&](int tiles) { return wave_reduce(blocks_walking(mine, shift, tiles, causal), [](int a, int b) { return a + b; }); };
     if (!divide(count(0))) return false;
-    const int slot = work.slot;
     // The most tiles of which more than `slot` blocks have as many.
-    const unsigned keys = few ? wave_reduce(mine.k_len, [](int a, int b) { return max(a, b); }) : p.k_tokens;
+    const unsigned keys = wave_reduce(mine.k_len, [](int a, int b) { return max(a, b); });
     int low = 0, high = static_cast<int>((keys + kTileKeys - 1) / kTileKeys) + 1;
     while (high - low > 1) {
         const int middle = (low + high) >> 1;
-        if (count(middle) > slot)
+        if (count(middle) > work.slot)
             low = middle;
         else
             high = middle;
     }
-    int rest = slot - count(low + 1);  // among the blocks of exactly `low` tiles
-    for (int base = 0; base < p.batch; base += kWave) {
-        const int b = base + lane;
-        Sequence s = mine;
-        if (base) s = b < p.batch ? sequence_at(p, b) : Sequence{0, 0, 0, 0};
-        const int above = blocks_walking(s, shift, low + 1, causal);
-        const int here = blocks_walking(s, shift, low, causal) - above;
-        const int before = static_cast<int>(prefix_sum(here));
-        const std::uint64_t past = __ballot(before > rest);
-        if (past) {
-            const int at = __builtin_ctzll(past);
-            found.q0 = __builtin_amdgcn_readlane(s.q0, at);
-            found.q_len = __builtin_amdgcn_readlane(s.q_len, at);
-            found.k0 = __builtin_amdgcn_readlane(s.k0, at);
-            found.k_len = __builtin_amdgcn_readlane(s.k_len, at);
-            // Blocks of a sequence walk more tiles the later they are.
-            const int blocks = blocks_walking(found, shift, 0, causal);
-            work.block = blocks - 1 - __builtin_amdgcn_readlane(above, at) - (rest - __builtin_amdgcn_readlane(before - here, at));
-            return true;
-        }
-        rest -= __builtin_amdgcn_readlane(before, kWave - 1);
-    }
-    return false;  // (the starts changed meanwhile)
+    // Among the blocks of exactly `low` tiles.
+    const int above = blocks_walking(mine, shift, low + 1, causal), here = blocks_walking(mine, shift, low, causal) - above;
+    const int before = static_cast<int>(prefix_sum(here));
+    const int rest = work.slot - wave_reduce(above, [](int a, int b) { return a + b; });
+    const int at = __builtin_ctzll(__ballot(before > rest));
+    found.q0 = __builtin_amdgcn_readlane(mine.q0, at);
+    found.q_len = __builtin_amdgcn_readlane(mine.q_len, at);
+    found.k0 = __builtin_amdgcn_readlane(mine.k0, at);
+    found.k_len = __builtin_amdgcn_readlane(mine.k_len, at);
+    // Blocks of a sequence walk more tiles the later they are.
+    work.block = blocks_walking(found, shift, 0, false) - 1 - __builtin_amdgcn_readlane(above, at) -
+                 (rest - __builtin_amdgcn_readlane(before - here, at));
+    return true;
 }
 
 // ------------------------------------------------------- 16-bit arithmetic
@@ -737,9 +744,9 @@ extern "C" int tilemix_attention_packed(const TileMixPackedAttentionArgs* args, 
     p.causal = a.causal != 0;
     p.negate = a.score_scale < 0.0f;
     p.score_log2 = std::min(std::fabs(a.score_scale) * kLog2e, FLT_MAX);  // finite: a score of 0 stays 0
-    // Blocks of all sequences: each has at most one that is not full.
+    // Blocks of all sequences: each has at most one that is not full (find_work: and, of many, one number).
     const int tokens = kBlockRows >> p.team_shift;
-    const std::int64_t blocks = a.q_tokens / tokens + static_cast<std::int64_t>(std::min(a.batch, a.q_tokens));
+    const std::int64_t blocks = a.q_tokens / tokens + static_cast<std::int64_t>(a.batch > kWave ? a.batch : std::min(a.batch, a.q_tokens));
     const std::int64_t grid = blocks * p.kv_heads * p.chunks;
     if (grid > 0xffffffffLL / kThreadsPerGroup) return hipErrorInvalidConfiguration;  // threads of a launch
     int units = 0;
