@@ -60,6 +60,7 @@ struct PackedParams {
     int causal;
     int negate;  // score_scale < 0: Q is negated
     float score_log2;  // |score_scale| log2(e)
+    int longest_first;
     int places;        // workgroups of a team that share its blocks' key tiles; 0: one each
     // Of a split call: a workspace of the library.
     float* part_o;
@@ -130,10 +131,10 @@ struct Work {
 // The work of place number `place` of a team, false past the last. kSplit: the team's
 // `places` are dealt out to its blocks. Wave-uniform.
 //
-// Up to 64 sequences, one a lane: blocks of more key tiles first (the last to start are the
-// shortest; a long walk that starts last would run alone), found by a search over tile
-// counts. More sequences keep their order, as every step of that search would read all of
-// their lengths (1000 sequences of 50 tokens, 32 heads: 707 us, 150 so): sequence b's blocks
+// Up to 64 sequences, one a lane: in order where all blocks start at once, else blocks of more
+// key tiles first (the last to start are the shortest; a long walk that starts last would run
+// alone), found by a search over tile counts. More sequences keep their order, as
+// every step of that search would read all of their lengths (1000 sequences of 50 tokens, 32 heads: 707 us, 150 so): sequence b's blocks
 // have the numbers from floor(start / tokens of a block) + b on, which leaves room for
 // all of them, and is found by a search over the starts. Numbers left over have no work.
 template <bool kSplit>
@@ -170,25 +171,32 @@ __device__ __forceinline__ bool find_work(const PackedParams& p, int place, int 
         work.block = blocks_walking(found, shift, 0, false) - 1 - (work.slot - number_of(low));
         return work.block >= 0;
     }
-    const bool causal = p.causal != 0;
     Sequence mine{0, 0, 0, 0};
     if (lane < p.batch) mine = sequence_at(p, lane);
-    auto count = [&](int tiles) { return wave_reduce(blocks_walking(mine, shift, tiles, causal), [](int a, int b) { return a + b; }); };
-    if (!divide(count(0))) return false;
-    // The most tiles of which more than `slot` blocks have as many.
-    const unsigned keys = wave_reduce(mine.k_len, [](int a, int b) { return max(a, b); });
-    int low = 0, high = static_cast<int>((keys + kTileKeys - 1) / kTileKeys) + 1;
-    while (high - low > 1) {
-        const int middle = (low + high) >> 1;
-        if (count(middle) > work.slot)
-            low = middle;
-        else
-            high = middle;
+    // Blocks that come before the slot: `above` of the lane's, and among `here` those of the lanes before.
+    int above = 0, here = blocks_walking(mine, shift, 0, false);
+    int before = static_cast<int>(prefix_sum(here));
+    if (!divide(__builtin_amdgcn_readlane(before, kWave - 1))) return false;
+    int rest = work.slot;
+    if (p.longest_first) {
+        const bool causal = p.causal != 0;
+        auto sum = [](int v) { return wave_reduce(v, [](int a, int b) { return a + b; }); };
+        // The most tiles of which more than `slot` blocks have as many.
+        const unsigned keys = wave_reduce(mine.k_len, [](int a, int b) { return max(a, b); });
+        int low = 0, high = static_cast<int>((keys + kTileKeys - 1) / kTileKeys) + 1;
+        while (high - low > 1) {
+            const int middle = (low + high) >> 1;
+            if (sum(blocks_walking(mine, shift, middle, causal)) > work.slot)
+                low = middle;
+            else
+                high = middle;
+        }
+        // Among the blocks of exactly `low` tiles.
+        above = blocks_walking(mine, shift, low + 1, causal);
+        here = blocks_walking(mine, shift, low, causal) - above;
+        before = static_cast<int>(prefix_sum(here));
+        rest -= sum(above);
     }
-    // Among the blocks of exactly `low` tiles.
-    const int above = blocks_walking(mine, shift, low + 1, causal), here = blocks_walking(mine, shift, low, causal) - above;
-    const int before = static_cast<int>(prefix_sum(here));
-    const int rest = work.slot - wave_reduce(above, [](int a, int b) { return a + b; });
     const int at = __builtin_ctzll(__ballot(before > rest));
     found.q0 = __builtin_amdgcn_readlane(mine.q0, at);
     found.q_len = __builtin_amdgcn_readlane(mine.q_len, at);
@@ -754,6 +762,9 @@ extern "C" int tilemix_attention_packed(const TileMixPackedAttentionArgs* args, 
     if (found != hipSuccess) return found;
     const bool bf16 = a.dtype == TILEMIX_DTYPE_BF16;
     const hipStream_t s = static_cast<hipStream_t>(stream);
+    // The order matters to more than one round of workgroups (4 x 2048 tokens, 16 heads x 64: in
+    // order 59 us, longest first 52), the search's time to the rest (4 x 250: 8.7 us with it, 8.0).
+    p.longest_first = grid > 2 * units;
     // Few blocks with long walks are split, into as many workgroups as are resident at
     // once. The lengths are not known here, so the average walk decides (2 x 256 tokens, 16 heads
     // x 128; in one piece and split): 6 tiles 17.7 and 19.8 us, 10 22.9 and 23.1, 18 33.6 and
@@ -763,6 +774,7 @@ extern "C" int tilemix_attention_packed(const TileMixPackedAttentionArgs* args, 
     const double walk = (p.causal ? keys - 0.5 * std::min(rows, keys) : keys) / kTileKeys;
     if (blocks <= places && 2 * ((rows + tokens - 1) / tokens) * a.batch <= static_cast<double>(places) && walk >= kSplitWalk) {
         p.places = static_cast<int>(places);
+        p.longest_first = 0;
         SplitCall call{p, bf16, places * teams, s};
         bool given = false;
         const hipError_t status = call_with_workspace(
