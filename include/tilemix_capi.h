@@ -287,8 +287,8 @@ int tilemix_quantize_qk_strided(const uint16_t* Q, const uint16_t* K, int8_t* Q8
  * sees no key becomes 0; rows of O outside every sequence are left as they were.
  * Keys and values that a row does not see do not reach it, whatever they hold.
  * Starts do not decrease. (Whatever they hold, they are clamped to 0 ..
- * q_tokens / k_tokens, and a sequence that would end before it starts is empty; of
- * more than 64 sequences some may then be left out.) q_tokens or batch 0: nothing to do. k_row_stride and
+ * q_tokens / k_tokens, and a sequence that would end before it starts is empty;
+ * others' rows may then be left out.) q_tokens or batch 0: nothing to do. k_row_stride and
  * v_row_stride up to 2^24 elements (more: NotSupported); 2^24 blocks of 128
  * rows (tokens x heads) or more -> InvalidConfiguration.
  * A call of few rows with many keys has its key ranges split over several

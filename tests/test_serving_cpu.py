@@ -145,6 +145,16 @@ def test_rows_in_place_have_one_layout(tm):
         assert code("append", **other) == INVALID, other
 
 
+def test_host_tensors_are_refused(tm):
+    import torch
+
+    host = torch.zeros(64, dtype=torch.float16)
+    for kind, names in (("packed", ("Q", "q_starts")), ("append", ("K", "slots", "cos_sin")), ("gather", ("K_out", "cache")),
+                        ("decode", ("lengths", "workspace", "O"))):
+        for name in names:
+            assert code(kind, **{name: host}) == INVALID, (kind, name)
+
+
 def test_calls_with_nothing_to_do(tm):
     """No device is asked for: they succeed on a machine without a GPU."""
     assert code("packed", batch=0) == 0 and code("packed", q_tokens=0, Q=None, O=None) == 0

@@ -1,6 +1,7 @@
 """Serving entry points of include/tilemix_capi.h: attention of packed sequences
 and the paged 4-bit key/value cache. Like the rest of the binding they take torch
-device tensors (or raw addresses, ``None`` for NULL) and return the hipError_t code;
+device tensors (or raw addresses, ``None`` for NULL), of the current device (others:
+InvalidValue), and return the hipError_t code;
 sizes, layouts and errors are those of the C header. Strides count elements, 0 =
 dense [tokens, heads, d].
 """
@@ -8,11 +9,12 @@ from __future__ import annotations
 
 import ctypes
 import struct
+import sys
 from dataclasses import dataclass
 from operator import attrgetter
 from typing import Any
 
-from .api import _stream, library
+from .api import ERROR_INVALID_VALUE, _stream, library
 
 _vp, _int, _i64, _sz, _f32 = ctypes.c_void_p, ctypes.c_int, ctypes.c_int64, ctypes.c_size_t, ctypes.c_float
 
@@ -50,7 +52,7 @@ class _Entry:
     """An entry point that takes a structure, packed from the fields of the same names of a
     dataclass. The fields are fetched in one call and the bound function is kept, as a decode
     step's kernels are not much longer than the call (of 31 fields: 4.4 us with a ctypes
-    structure filled from them, 2.3 us so)."""
+    structure filled from them, 2.4 us so, and 0.6 us for the tensors' devices)."""
 
     _CODES = {_vp: "P", _int: "i", _i64: "q", _sz: "N", _f32: "f"}
 
@@ -71,7 +73,21 @@ class _Entry:
             self._function = function
         values = self._fetch(args)
         n = self._pointers
-        pointers = [0 if x is None else x if x.__class__ is int else x.data_ptr() for x in values[:n]]
+        # A kernel of the current device would fault on another's memory, or the host's (device -1).
+        pointers, device = [], None
+        for x in values[:n]:
+            if x is None:
+                pointers.append(0)
+            elif x.__class__ is int:
+                pointers.append(x)
+            else:
+                if device is None:
+                    device = x.get_device()
+                    if device < 0 or device != sys.modules["torch"].cuda.current_device():
+                        return ERROR_INVALID_VALUE
+                elif x.get_device() != device:
+                    return ERROR_INVALID_VALUE
+                pointers.append(x.data_ptr())
         return self._function(self._pack(*pointers, *values[n:]), _stream(stream))
 
 
