@@ -486,6 +486,7 @@ def test_captured_step_takes_lengths_and_slots_at_replay(tm, cuda):
 LARGE_DECODES = [
     _decode([(37 * i * i) % 2500 for i in range(80)], heads=(8, 2), size=64), _decode([3000, 1, 0, 900, 2047], heads=(32, 2), d=128, size=128, dtype="bf16"),
     _decode([9000], heads=(1, 1), d=128, size=32), _decode([1024] * 6, heads=(4, 4), d=72, size=64, dtype="bf16"),
+    _decode([200] * 400, heads=(4, 4), dtype="bf16"), _decode([100] * 200, heads=(4, 4), d=128), _decode([700] * 100, heads=(12, 4)),
     _decode([300 + 7 * i for i in range(40)], heads=(20, 1), size=96, table_pad=2), _decode([31] * 300, heads=(2, 2), d=128),
 ]
 

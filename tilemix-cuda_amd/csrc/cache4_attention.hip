@@ -18,7 +18,7 @@
 // does not fit beside the accumulators without spills.)
 //
 // Split of the work: the blocks of all sequences and heads, one after the other, are
-// cut into ranges of equal length, one per workgroup (at most two a CU, one round),
+// cut into ranges of equal length, one per workgroup (two or three a CU, one round),
 // found on the device from the lengths (first_segment): lengths differ, and the host does not
 // know them. A range is a series of segments - blocks of one sequence and head; a
 // segment's queries and first blocks are on their way while the one before is merged over
@@ -26,8 +26,8 @@
 // head: those go to the workspace, where the workgroup that arrives last merges them in order.
 //
 // Measured: 64 sequences of 1 to 16384 tokens, 32 query and 8 key heads x 128: 93 us, 4.5 TB/s;
-// 2 of 32768 tokens, 16 heads: 35 us, 4.3 TB/s; 64 of 8192 tokens, 8 key heads, 5.2 TB/s. A
-// range's start and end take about 6 us, a step to another sequence 4.6. One sequence of 1003
+// 2 of 32768 tokens, 16 heads: 36 us, 4.2 TB/s; 64 of 8192 tokens, 8 key heads, 5.2 TB/s. A
+// range's start and end take about 6 us. One sequence of 1003
 // tokens, 4 key heads x 64: 9.7 us.
 
 #include "attention_common.h"
@@ -44,12 +44,15 @@ namespace {
 
 constexpr int kWaves = 4;
 constexpr int kThreads = kWaves * kWave;
-constexpr int kGroupsPerUnit = 2;  // workgroups of a CU that registers are allocated for
-constexpr int kSlots = 2;         // blocks in a wave's ring: one computed, the others under way
-constexpr int kTileRows = 16;     // query rows of a workgroup
-constexpr int kLeastSteps = 8;   // places of a range at least
-constexpr int kSwitch = 8;       // places of a range that the step to another sequence counts for
-constexpr int kRanges = 512;    // at most: workgroups that the device holds at once
+// Workgroups of a CU: three of 8 rows (their LDS is just under a third), two of 16. (128
+// sequences of up to 200 tokens, 8 key heads x 128: two 23 us, three 20; of up to 2048 41 and 38; two of
+// 32768, 16 heads, 35.7 and 36.4.)
+constexpr int groups_per_unit(int rows) { return rows == 8 ? 3 : 2; }
+constexpr int kSlots = 2;       // blocks in a wave's ring, the one computed and the next (three: 0 to 6 % more time)
+constexpr int kTileRows = 16;   // query rows of a workgroup
+constexpr int kLeastSteps = 8;  // places of a range at least
+constexpr int kSwitch = 8;      // places of a range that the step to another sequence counts for
+constexpr int kRanges = 768;    // at most: workgroups that the device holds at once
 // The workspace: arrival counters, then rows of O and their states for the two parts
 // (one continued, one to be continued) that a range can have.
 constexpr std::size_t kWorkspaceBytes =
@@ -185,19 +188,23 @@ __device__ __forceinline__ bool first_segment(const DecodeParams& p, int range, 
     // 1024 blocks, ranges of 8 places: 22.7 us, 22 19.0, 32 19.7; of 128, 8 places 12.0, 16 13.0).
     const int least = max(static_cast<int>(sqrtf(0.5f * static_cast<float>(one) / static_cast<float>(p.batch))), kLeastSteps);
     plan.length = max(static_cast<int>((total + p.ranges - 1) / p.ranges), least);
-    const unsigned items = p.batch * heads;
-    if (alike && items <= static_cast<unsigned>(p.ranges)) {
-        // Each sequence and head in as many whole ranges as there are for it, if that is
-        // hardly more for each: no range then has parts of two, which takes it longer (2
-        // sequences of 32768 tokens, 16 heads: 40.7 us, 35.4 so).
-        const unsigned each = p.ranges / items;
+    const unsigned items = p.batch * heads, ranges = p.ranges;
+    // Sequences that are all alike: whole ranges for each sequence and head, or whole sequences for
+    // a range, so that no range ends inside one, if that is hardly more for each or leaves at
+    // least two of three workgroups (2 sequences of 32768 tokens, 16 heads: 40.7 us cut anywhere,
+    // 35.4 so; 64 of 2048, 8 heads: 37.8 and 33.2; 128, 8 heads, of 1024: 43.0 and 37.7).
+    if (alike && items <= ranges) {
+        const unsigned each = ranges / items;
         const int length = max(static_cast<int>((sequence0 + each - 1) / each), least);
-        if (length <= plan.length + kSwitch) {
+        if (length <= plan.length + kSwitch || 3 * items * each >= 2 * ranges) {
             plan.gap = (length - sequence0 % length) % length;
             plan.length = length;
             one = blocks + p.batch * plan.gap;
             total = one * heads;
         }
+    } else if (alike) {
+        const unsigned each = (items - 1) / ranges + 1;
+        if (3 * ((items - 1) / each + 1) >= 2 * ranges) plan.length = each * (sequence0 + kSwitch);
     }
     const unsigned begin = static_cast<unsigned>(range) * plan.length;
     if (begin >= total) return false;
@@ -235,7 +242,7 @@ __device__ __forceinline__ void load_dwords_to_lds(int4v rsrc, unsigned lds_addr
 // 16 rows), and its scale and minimum once; with 8 rows the two halves of a
 // tile are the same rows, and hold the two 16-token halves of a block.
 template <int kGroups, bool kBf16, int kRows>
-__global__ __launch_bounds__(kThreads, kGroupsPerUnit) void cache4_attention_kernel(const DecodeParams p) {
+__global__ __launch_bounds__(kThreads, groups_per_unit(kRows)) void cache4_attention_kernel(const DecodeParams p) {
     constexpr int kTiles = kRows / 8;  // tokens of a lane
     constexpr int kDP = 64 * kGroups;
     constexpr int kBlockBytes = cache_block_bytes(kGroups);
@@ -246,8 +253,8 @@ __global__ __launch_bounds__(kThreads, kGroupsPerUnit) void cache4_attention_ker
     constexpr int kPieceBytes = kRows * kDP * 4;
     static_assert(kPieceBytes >= kGroups * 2 * kRows * kCacheKeys * 2, "p scale fits");
     __shared__ __attribute__((aligned(16))) unsigned char lds_piece[kWaves][kPieceBytes];
-    __shared__ __attribute__((aligned(16))) float lds_ml[kWaves][kTileRows][4];  // maximum, sum, sum p minimum of both groups
-    __shared__ int lds_last[2];
+    __shared__ __attribute__((aligned(16))) float lds_ml[kWaves][kRows][4];  // maximum, sum, sum p minimum of both groups
+    int* const lds_last = reinterpret_cast<int*>(&lds_ml[0][0][0]);  // [2], at the end
 
     const int tid = threadIdx.x;
     const int lane = tid & (kWave - 1);
@@ -815,9 +822,11 @@ extern "C" int tilemix_attention_cache4(const TileMixCache4AttentionArgs* args, 
     // Places of one of them, and its end rounded up to a range's length.
     const std::int64_t most = 2 * ((p.most_tokens - 1) / kCacheKeys + 1 + kSwitch);
     if (items > 0x3fffffffLL / most) return hipErrorInvalidConfiguration;
-    p.ranges = static_cast<int>(std::min<std::int64_t>(kRanges, (items * most - 1) / kLeastSteps + 1));
-    const hipError_t found = check_device();
+    int units = 0;
+    const hipError_t found = check_device(&units);
     if (found != hipSuccess) return found;
+    const int held = std::min(kRanges, groups_per_unit(p.group <= 8 ? 8 : 16) * units);
+    p.ranges = static_cast<int>(std::min<std::int64_t>(held, (items * most - 1) / kLeastSteps + 1));
     const hipStream_t s = static_cast<hipStream_t>(stream);
     const bool bf16 = a.dtype == TILEMIX_DTYPE_BF16;
     const unsigned workgroups = static_cast<unsigned>(p.ranges);
