@@ -23,7 +23,6 @@ and code = (x - minimum) / scale rounded to even.
 """
 from __future__ import annotations
 
-import functools
 import math
 import random
 import sys
@@ -38,7 +37,6 @@ WORKSPACE = 16 << 20  # bytes a serving program keeps for its decode calls
 KEYS = 32  # tokens of a cache block
 
 
-@functools.cache
 def _tilemix():
     package = str(Path.cwd() / "tilemix-cuda_amd")
     if package not in sys.path:
