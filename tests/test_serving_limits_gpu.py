@@ -1,0 +1,54 @@
+"""The serving operators at the edges of what their entry points take: pages past
+2 GiB, wide page tables, sequences of nearly 2^31 keys, values near the ends of
+their types.
+"""
+from __future__ import annotations
+
+import numpy as np
+import pytest
+import torch
+
+import serving_reference as ref
+from test_cache4_gpu import DT, _check, _code, _decode, _decode_expected, _read_rows, _write_rows
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture(scope="module")
+def workspace(tm, cuda):
+    return torch.zeros(tm.attention_cache4_workspace_bytes(), dtype=torch.uint8, device="cuda")
+
+
+@pytest.mark.parametrize("d,blocks,dtype", [(128, 470_000, "f16"), (40, 940_000, "bf16")])
+def test_one_page_past_2_gib(tm, cuda, workspace, d, blocks, dtype):
+    """A contiguous cache of one page a sequence: its last blocks lie 2.17 GB from its first.
+    All tokens before the last 90 are zeros, whose scores of 0 have no weight beside 50 and more."""
+    size, tokens = 32 * blocks, 90
+    cache = torch.zeros(tm.cache4_bytes(2, size, 1, d), dtype=torch.uint8, device="cuda")
+    assert cache.numel() // 2 > 2 ** 31
+    gen = torch.Generator().manual_seed(d)
+    base = torch.randn(1, 1, d, generator=gen)
+    k = (base + 0.1 * torch.randn(tokens, 1, d, generator=gen)).to(DT[dtype])
+    v = torch.randn(tokens, 1, d, generator=gen).to(DT[dtype])
+    q = (base + 0.1 * torch.randn(1, 2, d, generator=gen)).to(DT[dtype])
+    scale = 60.0 / float((base ** 2).sum())
+    slots = torch.arange(2 * size - tokens, 2 * size, device="cuda")  # the end of page 1
+    shape = dict(cache=cache, pages=2, page_size=size, kv_heads=1, d=d, dtype=_code(tm, dtype))
+    tm.check(tm.cache4_append(tm.Cache4AppendArgs(K=k.cuda(), V=v.cuda(), slots=slots, tokens=tokens, **shape)))
+    back = [torch.empty(tokens, 1, d, dtype=DT[dtype], device="cuda") for _ in "kv"]
+    tm.check(tm.cache4_gather(tm.Cache4GatherArgs(slots=slots, tokens=tokens, K_out=back[0], V_out=back[1], **shape)))
+    o = torch.full((1, 2, d), 9.0, dtype=DT[dtype], device="cuda")
+    tm.check(tm.attention_cache4(tm.Cache4AttentionArgs(
+        Q=q.cuda(), O=o, block_table=torch.tensor([[1]], dtype=torch.int32, device="cuda"),
+        lengths=torch.tensor([size], dtype=torch.int32, device="cuda"), workspace=workspace, workspace_bytes=workspace.numel(),
+        max_pages=1, batch=1, q_heads=2, score_scale=scale, **shape)))
+    torch.cuda.synchronize()
+    small, places = np.zeros((2, 1, 2, ref.block_bytes(d)), np.uint8), np.arange(tokens)
+    _write_rows(small, 64, places, k.float().numpy(), v.float().numpy())
+    for got, rows in zip(back, _read_rows(small, 64, places, d)):
+        assert torch.equal(got.cpu(), torch.from_numpy(rows).float().to(DT[dtype]))
+    c = _decode([tokens], heads=(2, 1), d=d, dtype=dtype, size=64, scale=scale)
+    scores = _read_rows(small, 64, places, d)[0][:, 0] @ q[0].double().numpy().T * scale
+    assert scores.max(0).min() > 50  # 3e7 zeros weigh under 3e7 e^-50 < 2^-46 of the row
+    expected, bound = _decode_expected(c, q, small, [places])
+    _check(o, expected, bound, "the end of the page")

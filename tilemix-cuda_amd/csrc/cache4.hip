@@ -89,7 +89,7 @@ __device__ __forceinline__ Place place_of(const Cache& cache, std::int64_t slot)
     at.ok = slot >= 0 && slot < cache.pages * cache.page_size;
     const std::int64_t page = at.ok ? slot / cache.page_size : 0;
     const int inside = at.ok ? static_cast<int>(slot - page * cache.page_size) : 0;
-    at.block = page * cache.page_bytes + static_cast<std::int64_t>(inside / kCacheKeys) * cache_block_bytes(cache.groups);
+    at.block = cache_block_at(page, cache.page_bytes, inside / kCacheKeys, cache_block_bytes(cache.groups));
     at.t = inside % kCacheKeys;
     return at;
 }

@@ -347,7 +347,7 @@ __global__ __launch_bounds__(kThreads, groups_per_unit(kRows)) void cache4_atten
             if (page - window >= kWave) load_window();
             const int number = __builtin_amdgcn_readlane(window_page, page - window);
             if (number >= 0 && number < p.cache.pages) {
-                data = head_data + number * p.cache.page_bytes + inside * kBlockBytes;
+                data = head_data + cache_block_at(number, p.cache.page_bytes, inside, kBlockBytes);
                 bytes = kBlockBytes;
                 return;
             }

@@ -67,6 +67,13 @@ struct Cache {
     int groups;
 };
 
+// Where a block lies: bytes from the cache's start (with head 0's part of the page; a head more is
+// head_bytes more). `block` is its number in the page. A head's part of a page may pass 2 GiB
+// (make_cache: head_bytes under 2^32), so that neither product fits 32 bits.
+__host__ __device__ inline std::int64_t cache_block_at(std::int64_t page, std::int64_t page_bytes, int block, int block_bytes) {
+    return page * page_bytes + static_cast<std::int64_t>(block) * block_bytes;
+}
+
 // TILEMIX_SUCCESS, or the error of the cache arguments.
 inline hipError_t make_cache(Cache& out, const std::uint8_t* data, std::int64_t pages, int page_size, int kv_heads, int d) {
     if (!data || reinterpret_cast<std::uintptr_t>(data) % 16 != 0 || pages <= 0 || pages > 0x7fffffffLL || page_size <= 0 ||
