@@ -55,9 +55,33 @@ void blocks_lie_inside_their_page() {
     }
 }
 
+// The last key that a row sees, for rows up to a workgroup's past a sequence's end and
+// lengths up to the largest.
+void rows_see_up_to_their_own_key() {
+    using namespace tilemix;
+    const int most = 0x7fffffff;
+    for (const int q_len : {1, 2, 31, 128, 129, 1 << 20, most - 128}) {
+        for (const int k_len : {0, 1, 5, 128, 1 << 20, most - 64, most - 31, most - 1, most}) {
+            const int context = k_len - q_len;
+            for (const int from : {0, q_len - 40, q_len - 1}) {
+                for (int row = from < 0 ? 0 : from; row < from + 128; ++row) {
+                    const long long end = row < q_len ? row : q_len - 1LL;
+                    const long long expected = static_cast<long long>(k_len) - q_len + end;
+                    if (last_seen(context, row, q_len) != expected) {
+                        std::printf("row %d of %d sees key %lld of %d, not %d\n", row, q_len, expected, k_len,
+                                    last_seen(context, row, q_len));
+                        ++failures;
+                    }
+                }
+            }
+        }
+    }
+}
+
 }  // namespace
 
 int main() {
+    rows_see_up_to_their_own_key();
     blocks_lie_inside_their_page();
     if (failures == 0) std::printf("serving rules OK\n");
     return failures ? 1 : 0;

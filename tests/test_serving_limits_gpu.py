@@ -52,3 +52,22 @@ def test_one_page_past_2_gib(tm, cuda, workspace, d, blocks, dtype):
     assert scores.max(0).min() > 50  # 3e7 zeros weigh under 3e7 e^-50 < 2^-46 of the row
     expected, bound = _decode_expected(c, q, small, [places])
     _check(o, expected, bound, "the end of the page")
+
+
+@pytest.mark.parametrize("last", [8.0, float("nan"), float("inf")])
+@pytest.mark.parametrize("heads", [1, 4])
+def test_a_sequence_of_nearly_2_31_keys(tm, cuda, last, heads):
+    """Row 1 of two sees the last of 2^31 - 1 keys, row 0 does not. All other keys and
+    values are zeros; the last key's score is 64, beside which 2^31 zeros weigh 2^-61."""
+    keys, d = 2 ** 31 - 1, 8
+    x = torch.zeros(keys, d, dtype=torch.float16, device="cuda")  # K and V alike
+    x[-1] = last
+    q = torch.ones(2, heads, d, dtype=torch.float16, device="cuda")
+    o = torch.full_like(q, 9.0)
+    starts = [torch.tensor([0, n], dtype=torch.int32, device="cuda") for n in (2, keys)]
+    tm.check(tm.attention_packed(tm.PackedAttentionArgs(
+        Q=q, K=x, V=x, O=o, q_starts=starts[0], k_starts=starts[1], batch=1, q_tokens=2, k_tokens=keys, q_heads=heads, kv_heads=1,
+        d=d, dtype=tm.DTYPE_F16, score_scale=1.0)))
+    torch.cuda.synchronize()
+    assert (o[0] == 0).all()
+    assert (o[1] == last).all() if last == 8.0 else torch.isnan(o[1]).all()

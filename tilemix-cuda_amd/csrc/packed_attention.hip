@@ -422,8 +422,7 @@ __global__ __launch_bounds__(kThreadsPerGroup, 2) void packed_attention_kernel(c
     st.m = -INFINITY;
 
     // Last key that some row of the workgroup / of the wave sees, and all rows of the wave see.
-    const int rows_end = min(t0 + tokens, seq.q_len);
-    const int group_last = p.causal ? min(context + rows_end, seq.k_len) - 1 : seq.k_len - 1;
+    const int group_last = p.causal ? last_seen(context, t0 + tokens - 1, seq.q_len) : seq.k_len - 1;
     const int all_tiles = group_last < 0 ? 0 : group_last / kTileKeys + 1;
     // Ranges of at least kLeastTiles tiles (one, of none, of a block without keys). A tile takes
     // 1.3 us, and the last workgroup merges a part in 0.8 us (latency of 64 KB): of n tiles,
@@ -435,8 +434,8 @@ __global__ __launch_bounds__(kThreadsPerGroup, 2) void packed_attention_kernel(c
     auto range_start = [&](int split) { return split * (all_tiles / splits) + min(split, all_tiles % splits); };
     const int first_tile = kSplit ? range_start(work.split) : 0;
     const int tiles = kSplit ? range_start(work.split + 1) : all_tiles;
-    const int wave_last = tw >= seq.q_len ? -1 : p.causal ? min(context + tw + kRowsPerWave, seq.k_len) - 1 : seq.k_len - 1;
-    const int all_last = p.causal ? context + tw : seq.k_len - 1;
+    const int wave_last = tw >= seq.q_len ? -1 : p.causal ? last_seen(context, tw + kRowsPerWave - 1, seq.q_len) : seq.k_len - 1;
+    const int all_last = p.causal ? last_seen(context, tw, seq.q_len) : seq.k_len - 1;
 
     // A row's probability of a key that it does not see is 0, but 0 times an infinite or NaN
     // value is NaN: such values are taken out of diagonal tiles, and put into the rows that
@@ -457,11 +456,11 @@ __global__ __launch_bounds__(kThreadsPerGroup, 2) void packed_attention_kernel(c
         issue_v(first_tile, 0);
     }
     for (int j = first_tile; j < tiles; ++j) {
-        const int k0 = j * kTileKeys;
+        const int k0 = j * kTileKeys, k_last = k0 + (kTileKeys - 1);  // (k0 + kTileKeys may be 2^31)
         tile_barrier();  // K_j, V_j landed; every wave finished P.V of the previous tile
         set_priority<2>();
         const bool active = k0 <= wave_last;
-        const bool masked = k0 + kTileKeys - 1 > min(all_last, seq.k_len - 1);
+        const bool masked = k_last > min(all_last, seq.k_len - 1);
         float16v s[2];
         float c = p.score_log2;
         if (active) {
@@ -484,7 +483,7 @@ __global__ __launch_bounds__(kThreadsPerGroup, 2) void packed_attention_kernel(c
             }
         }
         // The last key that the lane's row sees, from the tile's first key of the lane.
-        int seen = (p.causal ? min(context + tw + q, seq.k_len - 1) : seq.k_len - 1) - k0 - 4 * h;
+        int seen = (p.causal ? last_seen(context, tw + q, seq.q_len) : seq.k_len - 1) - k0 - 4 * h;
         if (active && masked) {
             asm volatile("" : "+v"(seen));
 #pragma unroll
@@ -494,7 +493,7 @@ __global__ __launch_bounds__(kThreadsPerGroup, 2) void packed_attention_kernel(c
                     s[kb][e] = 32 * kb + 8 * (e >> 2) + (e & 3) > seen ? -INFINITY : s[kb][e] * c;
             c = 1.0f;
         }
-        const bool diagonal = k0 + kTileKeys > first_hidden;  // of the workgroup
+        const bool diagonal = k_last >= first_hidden;  // of the workgroup
         unsigned char* const v_tile = lds_v + (v_buffer ? L::kVBytes : 0);
         constexpr int kChecks = kTileKeys * kChunks / kThreadsPerGroup;  // chunks of a thread
         auto checked = [&](int x) {

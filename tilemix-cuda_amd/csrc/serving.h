@@ -32,6 +32,13 @@ inline bool make_rows(Rows& out, const void* data, int tokens, int heads, int d,
     return strided_heads_ok(heads, std::max(tokens, 1), d, out.head, out.row);
 }
 
+// Causal rows are aligned at the end of their keys: row i of q_len sees keys 0 .. context + i,
+// context = k_len - q_len. The last key that row `row` sees; a row past the end sees what the
+// last one does, so that no sum passes 2^31 where k_len is just below it.
+__host__ __device__ inline int last_seen(int context, int row, int q_len) {
+    return context + (row < q_len ? row : q_len - 1);
+}
+
 // -------------------------------------------------------------- 4-bit cache
 
 // A block holds 32 tokens of one key head, in the order in which a wave of the
