@@ -175,3 +175,59 @@ def test_structures_match_the_header():
             kind, field = line.rsplit(None, 1) if "*" not in line else ("pointer", line.split("*")[1].strip())
             fields.append((field, ctypes.c_void_p if kind == "pointer" else kinds[kind]))
         assert [tuple(f) for f in structure._fields_] == fields, name
+
+
+class _DeviceTensor:
+    """What the binding asks of a tensor, as one of device 0 answers; its memory is never read."""
+
+    def __init__(self, dtype, contiguous=True, shape=(64,), strides=(1,)):
+        self.dtype, self._contiguous, self.shape, self._strides = dtype, contiguous, shape, strides
+
+    def get_device(self):
+        return 0
+
+    def data_ptr(self):
+        return X
+
+    def is_contiguous(self):
+        return self._contiguous
+
+    def stride(self, i=None):
+        return self._strides if i is None else self._strides[i]
+
+    def dim(self):
+        return len(self.shape)
+
+
+ROWS = "Q K V O Q_out K_out V_out".split()
+INDEX_TYPES = dict(q_starts="int32", k_starts="int32", token_positions="int32", block_table="int32", lengths="int32", slots="int64",
+                   cos_sin="float32")
+TENSORS = {"packed": "Q K V O q_starts k_starts", "append": "Q K V Q_out K_out cos_sin token_positions slots",
+           "gather": "slots K_out V_out", "decode": "Q O block_table lengths"}
+TENSORS = {kind: names.split() for kind, names in TENSORS.items()}
+
+
+def _with_tensors(monkeypatch, kind, **changed):
+    """The code of a call of device tensors of the right types but for `changed`."""
+    import torch
+
+    monkeypatch.setattr(torch.cuda, "current_device", lambda: 0)
+    call, args = CALLS[kind]
+    dtype = torch.bfloat16 if kind == "append" else torch.float16
+    tensors = {n: _DeviceTensor(getattr(torch, INDEX_TYPES[n]) if n in INDEX_TYPES else dtype) for n in TENSORS[kind]}
+    return call(args(**{**tensors, **changed}), stream=0)
+
+
+@pytest.mark.parametrize("kind", CALLS)
+def test_tensors_of_other_types_are_refused(tm, monkeypatch, kind):
+    import torch
+
+    if torch.cuda.is_available():
+        pytest.skip("the calls that pass the checks are stopped by the missing GPU")
+    for name in TENSORS[kind]:
+        right = {INDEX_TYPES[name]} if name in INDEX_TYPES else {"bfloat16" if kind == "append" else "float16", "int16", "uint16"}
+        for other in ("uint8", "int16", "uint16", "int32", "int64", "float16", "bfloat16", "float32", "float64"):
+            got = _with_tensors(monkeypatch, kind, **{name: _DeviceTensor(getattr(torch, other))})
+            assert (got != INVALID) == (other in right), (name, other, got)
+    if kind != "packed":
+        assert _with_tensors(monkeypatch, kind, cache=_DeviceTensor(torch.int32)) != INVALID  # bytes, whatever holds them

@@ -71,3 +71,28 @@ def test_a_sequence_of_nearly_2_31_keys(tm, cuda, last, heads):
     torch.cuda.synchronize()
     assert (o[0] == 0).all()
     assert (o[1] == last).all() if last == 8.0 else torch.isnan(o[1]).all()
+
+
+def test_tensors_of_other_types_are_refused(tm, cuda, workspace):
+    """Index tensors above all: a kernel takes narrower ones for as many values of its own."""
+    d, size = 64, 32
+    cache = torch.zeros(tm.cache4_bytes(2, size, 1, d), dtype=torch.uint8, device="cuda")
+    rows = {n: torch.ones(4, 1, d, dtype=torch.float16, device="cuda") for n in ("Q", "K", "V", "O")}
+    shape = dict(kv_heads=1, d=d, dtype=tm.DTYPE_F16)
+    paged = dict(cache=cache, pages=2, page_size=size)
+    int32 = torch.tensor([0, 1, 2, 3, 4], dtype=torch.int32, device="cuda")
+    append = dict(K=rows["K"], V=rows["V"], slots=int32[:4].long(), tokens=4, **paged, **shape)
+    gather = dict(slots=int32[:4].long(), K_out=rows["K"], V_out=rows["V"], tokens=4, **paged, **shape)
+    decode = dict(Q=rows["Q"], O=rows["O"], block_table=int32[:4].view(4, 1), lengths=int32[1:], workspace=workspace,
+                  workspace_bytes=workspace.numel(), max_pages=1, batch=4, q_heads=1, score_scale=1.0, **paged, **shape)
+    packed = dict(Q=rows["Q"], K=rows["K"], V=rows["V"], O=rows["O"], q_starts=int32, k_starts=int32, batch=4, q_tokens=4, k_tokens=4,
+                  q_heads=1, score_scale=1.0, **shape)
+    for call, args, fields, names in (
+            (tm.cache4_append, tm.Cache4AppendArgs, append, "K V slots"), (tm.cache4_gather, tm.Cache4GatherArgs, gather, "K_out V_out slots"),
+            (tm.attention_cache4, tm.Cache4AttentionArgs, decode, "Q O block_table lengths"),
+            (tm.attention_packed, tm.PackedAttentionArgs, packed, "Q K V O q_starts k_starts")):
+        tm.check(call(args(**fields)))
+        for name in names.split():
+            for other in (torch.uint8, torch.bfloat16, torch.float32, torch.int32 if name == "slots" else torch.int64):
+                assert call(args(**{**fields, name: fields[name].to(other)})) == 1, (name, other)
+    torch.cuda.synchronize()

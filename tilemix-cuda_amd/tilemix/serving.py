@@ -1,7 +1,7 @@
 """Serving entry points of include/tilemix_capi.h: attention of packed sequences
 and the paged 4-bit key/value cache. Like the rest of the binding they take torch
-device tensors (or raw addresses, ``None`` for NULL), of the current device (others:
-InvalidValue), and return the hipError_t code;
+device tensors (or raw addresses, ``None`` for NULL), of the current device and of the
+types that the header names (others: InvalidValue), and return the hipError_t code;
 sizes, layouts and errors are those of the C header. Strides count elements, 0 =
 dense [tokens, heads, d].
 """
@@ -14,7 +14,7 @@ from dataclasses import dataclass
 from operator import attrgetter
 from typing import Any
 
-from .api import ERROR_INVALID_VALUE, _stream, library
+from .api import DTYPE_BF16, DTYPE_F16, ERROR_INVALID_VALUE, _stream, library
 
 _vp, _int, _i64, _sz, _f32 = ctypes.c_void_p, ctypes.c_int, ctypes.c_int64, ctypes.c_size_t, ctypes.c_float
 
@@ -52,19 +52,38 @@ class _Entry:
     """An entry point that takes a structure, packed from the fields of the same names of a
     dataclass. The fields are fetched in one call and the bound function is kept, as a decode
     step's kernels are not much longer than the call (of 31 fields: 4.4 us with a ctypes
-    structure filled from them, 2.4 us so, and 0.6 us for the tensors' devices)."""
+    structure filled from them, 2.4 us so; the whole call with 9 tensors' devices and types 2.9)."""
+
+    # Types of what is not a tensor of the call's `dtype`. A kernel takes a tensor of narrower values for as many
+    # of its own, and would read past the end; the cache and the workspace are bytes, whatever holds them.
+    _TYPES = {**dict.fromkeys(("q_starts", "k_starts", "token_positions", "block_table", "lengths"), "int32"),
+              "slots": "int64", "cos_sin": "float32", "cache": None, "workspace": None}
 
     _CODES = {_vp: "P", _int: "i", _i64: "q", _sz: "N", _f32: "f"}
 
     def __init__(self, name: str, structure):
         names = [n for n, _ in structure._fields_]
+        self._names = names
         self._name, self._fetch, self._function = name, attrgetter(*names), None
         self._pointers = sum(1 for _, kind in structure._fields_ if kind is _vp)
+        self._dtype, self._known = names.index("dtype"), set()
         assert all(kind is _vp for _, kind in structure._fields_[:self._pointers])
         # Native sizes and alignment; a C structure also ends at a multiple of its alignment.
         packing = struct.Struct("@" + "".join(self._CODES[kind] for _, kind in structure._fields_) + "0P")
         assert packing.size == ctypes.sizeof(structure)
         self._pack = packing.pack
+
+    def _types_ok(self, dtype, types) -> bool:
+        """Whether a call of `dtype` takes tensors of these types (None: no tensor); 16-bit values also as bits."""
+        if (dtype, types) not in self._known:
+            torch = sys.modules["torch"]
+            rows = {DTYPE_F16: (torch.float16,), DTYPE_BF16: (torch.bfloat16,)}.get(dtype, ()) + (torch.int16, torch.uint16)
+            for name, found in zip(self._names, types):
+                wanted = self._TYPES.get(name, rows)
+                if found is not None and wanted is not None and found not in (wanted if wanted is rows else (getattr(torch, wanted),)):
+                    return False
+            self._known.add((dtype, types))
+        return True
 
     def __call__(self, args, stream) -> int:
         if self._function is None:
@@ -74,12 +93,11 @@ class _Entry:
         values = self._fetch(args)
         n = self._pointers
         # A kernel of the current device would fault on another's memory, or the host's (device -1).
-        pointers, device = [], None
+        pointers, types, device = [], [], None
         for x in values[:n]:
-            if x is None:
-                pointers.append(0)
-            elif x.__class__ is int:
-                pointers.append(x)
+            if x is None or x.__class__ is int:
+                pointers.append(x or 0)
+                types.append(None)
             else:
                 if device is None:
                     device = x.get_device()
@@ -88,7 +106,13 @@ class _Entry:
                 elif x.get_device() != device:
                     return ERROR_INVALID_VALUE
                 pointers.append(x.data_ptr())
-        return self._function(self._pack(*pointers, *values[n:]), _stream(stream))
+                types.append(x.dtype)
+        if device is not None and not self._types_ok(values[self._dtype], tuple(types)):
+            return ERROR_INVALID_VALUE
+        packed = self._pack(*pointers, *values[n:])
+        if stream is None and device is not None:  # as _stream, with the device known
+            return self._function(packed, sys.modules["torch"]._C._cuda_getCurrentRawStream(device))
+        return self._function(packed, _stream(stream))
 
 
 @dataclass
