@@ -231,3 +231,35 @@ def test_tensors_of_other_types_are_refused(tm, monkeypatch, kind):
             assert (got != INVALID) == (other in right), (name, other, got)
     if kind != "packed":
         assert _with_tensors(monkeypatch, kind, cache=_DeviceTensor(torch.int32)) != INVALID  # bytes, whatever holds them
+
+
+@pytest.mark.parametrize("kind", CALLS)
+def test_tensors_of_other_layouts_are_refused(tm, monkeypatch, kind):
+    """What a call has no stride for is read as it lies: a view with gaps would be other values."""
+    import torch
+
+    if torch.cuda.is_available():
+        pytest.skip("the calls that pass the checks are stopped by the missing GPU")
+    types = {**{n: t for n, t in INDEX_TYPES.items() if n != "block_table"}, "cache": "uint8", "workspace": "uint8"}
+    for name in [n for n in TENSORS[kind] if n in types] + {"packed": [], "decode": ["cache", "workspace"]}.get(kind, ["cache"]):
+        for contiguous in (True, False):
+            got = _with_tensors(monkeypatch, kind, **{name: _DeviceTensor(getattr(torch, types[name]), contiguous=contiguous)})
+            assert (got != INVALID) == contiguous, (name, contiguous)
+    for name in set(TENSORS[kind]) & set(ROWS):  # these have strides of their own
+        dtype = torch.bfloat16 if kind == "append" else torch.float16
+        assert _with_tensors(monkeypatch, kind, **{name: _DeviceTensor(dtype, contiguous=False)}) != INVALID
+
+
+def test_rows_of_a_block_table_are_as_far_apart_as_the_call_says(tm, monkeypatch):
+    import torch
+
+    if torch.cuda.is_available():
+        pytest.skip("the calls that pass the checks are stopped by the missing GPU")
+
+    def table(strides, **options):
+        tensor = _DeviceTensor(torch.int32, contiguous=False, shape=(2,) * len(strides), strides=strides)
+        return _with_tensors(monkeypatch, "decode", block_table=tensor, **options) != INVALID  # batch 2, max_pages 2
+
+    assert table((2, 1)) and table((7, 1), table_stride=7) and table((7, 1), batch=1)
+    assert not table((7, 1)) and not table((2, 1), table_stride=7) and not table((1, 2)) and not table((14, 2), table_stride=14)
+    assert table((1, 5), max_pages=1) and table((5, 5), max_pages=1, table_stride=5) and not table((2,))

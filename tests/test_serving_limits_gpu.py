@@ -9,7 +9,7 @@ import pytest
 import torch
 
 import serving_reference as ref
-from test_cache4_gpu import DT, _check, _code, _decode, _decode_expected, _read_rows, _write_rows
+from test_cache4_gpu import DT, _check, _code, _decode, _decode_args, _decode_expected, _decode_problem, _queries, _read_rows, _write_rows
 
 pytestmark = pytest.mark.gpu
 
@@ -95,4 +95,22 @@ def test_tensors_of_other_types_are_refused(tm, cuda, workspace):
         for name in names.split():
             for other in (torch.uint8, torch.bfloat16, torch.float32, torch.int32 if name == "slots" else torch.int64):
                 assert call(args(**{**fields, name: fields[name].to(other)})) == 1, (name, other)
+    torch.cuda.synchronize()
+
+
+def test_index_tensors_with_gaps_are_refused(tm, cuda, workspace):
+    c = _decode([40, 70], heads=(2, 1), d=64)
+    cache, table, _, pages = _decode_problem(c)
+    q = _queries(c).cuda()
+    args = _decode_args(tm, c, q, torch.empty_like(q), cache, table, pages, workspace)
+    tm.check(tm.attention_cache4(args))
+
+    def refused(**changed):
+        return tm.attention_cache4(tm.Cache4AttentionArgs(**{**args.__dict__, **changed})) == 1
+
+    assert refused(lengths=args.lengths.repeat_interleave(2)[::2])
+    wide = torch.zeros(2, table.shape[1] + 2, dtype=torch.int32, device="cuda")
+    wide[:, :table.shape[1]] = args.block_table
+    assert refused(block_table=wide[:, :table.shape[1]]) and refused(block_table=wide.t().contiguous().t()[:, :table.shape[1]])
+    assert not refused(block_table=wide[:, :table.shape[1]], table_stride=wide.shape[1])
     torch.cuda.synchronize()

@@ -1,9 +1,11 @@
 """Serving entry points of include/tilemix_capi.h: attention of packed sequences
 and the paged 4-bit key/value cache. Like the rest of the binding they take torch
 device tensors (or raw addresses, ``None`` for NULL), of the current device and of the
-types that the header names (others: InvalidValue), and return the hipError_t code;
-sizes, layouts and errors are those of the C header. Strides count elements, 0 =
-dense [tokens, heads, d].
+types that the header names, and return the hipError_t code; sizes, layouts and errors
+are those of the C header. Strides count elements, 0 = dense [tokens, heads, d]; what has
+no stride in the call (starts, lengths, slots, positions, the table of angles, the cache,
+the workspace) is contiguous, and the rows of a block table lie as far apart as the call
+says. Other devices, types and layouts: InvalidValue.
 """
 from __future__ import annotations
 
@@ -52,12 +54,13 @@ class _Entry:
     """An entry point that takes a structure, packed from the fields of the same names of a
     dataclass. The fields are fetched in one call and the bound function is kept, as a decode
     step's kernels are not much longer than the call (of 31 fields: 4.4 us with a ctypes
-    structure filled from them, 2.4 us so; the whole call with 9 tensors' devices and types 2.9)."""
+    structure filled from them, 2.4 us so; the whole call with 9 tensors' devices, types and layouts 3.3)."""
 
     # Types of what is not a tensor of the call's `dtype`. A kernel takes a tensor of narrower values for as many
     # of its own, and would read past the end; the cache and the workspace are bytes, whatever holds them.
     _TYPES = {**dict.fromkeys(("q_starts", "k_starts", "token_positions", "block_table", "lengths"), "int32"),
               "slots": "int64", "cos_sin": "float32", "cache": None, "workspace": None}
+    _DENSE = {"q_starts", "k_starts", "token_positions", "lengths", "slots", "cos_sin", "cache", "workspace"}
 
     _CODES = {_vp: "P", _int: "i", _i64: "q", _sz: "N", _f32: "f"}
 
@@ -67,6 +70,8 @@ class _Entry:
         self._name, self._fetch, self._function = name, attrgetter(*names), None
         self._pointers = sum(1 for _, kind in structure._fields_ if kind is _vp)
         self._dtype, self._known = names.index("dtype"), set()
+        self._dense = [i for i, n in enumerate(names) if n in self._DENSE]
+        self._table = attrgetter("block_table", "table_stride", "max_pages", "batch") if "block_table" in names else None
         assert all(kind is _vp for _, kind in structure._fields_[:self._pointers])
         # Native sizes and alignment; a C structure also ends at a multiple of its alignment.
         packing = struct.Struct("@" + "".join(self._CODES[kind] for _, kind in structure._fields_) + "0P")
@@ -83,6 +88,20 @@ class _Entry:
                 if found is not None and wanted is not None and found not in (wanted if wanted is rows else (getattr(torch, wanted),)):
                     return False
             self._known.add((dtype, types))
+        return True
+
+    def _layouts_ok(self, args, values) -> bool:
+        for i in self._dense:
+            x = values[i]
+            if x is not None and x.__class__ is not int and not x.is_contiguous():
+                return False
+        if self._table is not None:
+            table, row, pages, batch = self._table(args)
+            if table is not None and table.__class__ is not int:
+                if table.dim() != 2:
+                    return table.is_contiguous()
+                between, step = table.stride()
+                return (step == 1 or pages == 1) and (between == (row or pages) or batch <= 1)
         return True
 
     def __call__(self, args, stream) -> int:
@@ -107,7 +126,7 @@ class _Entry:
                     return ERROR_INVALID_VALUE
                 pointers.append(x.data_ptr())
                 types.append(x.dtype)
-        if device is not None and not self._types_ok(values[self._dtype], tuple(types)):
+        if device is not None and not (self._types_ok(values[self._dtype], tuple(types)) and self._layouts_ok(args, values)):
             return ERROR_INVALID_VALUE
         packed = self._pack(*pointers, *values[n:])
         if stream is None and device is not None:  # as _stream, with the device known
