@@ -114,3 +114,29 @@ def test_index_tensors_with_gaps_are_refused(tm, cuda, workspace):
     assert refused(block_table=wide[:, :table.shape[1]]) and refused(block_table=wide.t().contiguous().t()[:, :table.shape[1]])
     assert not refused(block_table=wide[:, :table.shape[1]], table_stride=wide.shape[1])
     torch.cuda.synchronize()
+
+
+@pytest.mark.parametrize("c,past", [
+    (_decode([5000, 3, 0, 2300, 64], heads=(2, 1), d=64), 0), (_decode([2400] * 3 + [2399], heads=(8, 2), d=128, dtype="bf16"), 500),
+    (_decode([(13 * i) % 190 for i in range(90)], heads=(4, 2), d=72, size=64), 0), (_decode([4096, 100], heads=(20, 1), d=128, size=64), 1),
+    (_decode([160] * 70, heads=(4, 4), d=64, dtype="bf16"), 40)],
+    ids=lambda x: f"{len(x['lengths'])}x{max(x['lengths'])}" if isinstance(x, dict) else str(x))
+def test_block_tables_with_more_columns_than_the_call_has_pages(tm, cuda, workspace, c, past):
+    """A resident table of which a call uses the first max_pages columns: the others hold pages
+    of other sequences, which lengths `past` the call's pages must not reach."""
+    cache, table, slots, pages = _decode_problem(c)
+    max_pages = table.shape[1]
+    rng = np.random.default_rng(7)
+    wide = rng.integers(0, pages, (len(c["lengths"]), max_pages + 9)).astype(np.int32)
+    for b, n in enumerate(c["lengths"]):
+        need = (n + c["size"] - 1) // c["size"]
+        wide[b, :need] = table[b, :need]
+    q = _queries(c)
+    expected, bound = _decode_expected(c, q, cache, slots)
+    lengths = torch.tensor([n + past if n == max_pages * c["size"] else n for n in c["lengths"]], dtype=torch.int32, device="cuda")
+    assert past == 0 or int(lengths.max()) > max_pages * c["size"]
+    o = torch.full_like(q, 9.0).cuda()
+    args = _decode_args(tm, c, q.cuda(), o, cache, wide, pages, workspace, max_pages=max_pages, table_stride=wide.shape[1], lengths=lengths)
+    tm.check(tm.attention_cache4(args))
+    torch.cuda.synchronize()
+    _check(o, expected, bound, "wide table")
