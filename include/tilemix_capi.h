@@ -334,8 +334,8 @@ int tilemix_attention_packed(const TileMixPackedAttentionArgs* args, void* strea
  * the room of the next of these two). x is held as minimum + scale * code with
  *   minimum = bf16(least x) (a zero positive), scale = bf16((largest x - minimum) / 15),
  *   code = clamp(round_half_even((x - minimum) / scale), 0, 15),
- * 0 where scale is below 2^-100; a group with an infinite or NaN value (or
- * a range past fp32's) is held as NaN. Order inside a block, with B = ceil(d / 64):
+ * 0 where scale is below 2^-100; a group with an infinite or NaN value (or a
+ * range past fp32's, or a minimum past bf16's) is held as NaN. Order inside a block, with B = ceil(d / 64):
  *   key codes: 8 B words a token; features 64 m + 16 g + 8 w + e in word
  *     2 B g + 2 m + w, feature e (0 .. 7) at bits 4 (e / 2) + 16 (e % 2);
  *   value codes: [16 B][32 places] of 16 bits, features 4 q + f at bits 4 f of row q;

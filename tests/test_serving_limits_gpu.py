@@ -140,3 +140,29 @@ def test_block_tables_with_more_columns_than_the_call_has_pages(tm, cuda, worksp
     tm.check(tm.attention_cache4(args))
     torch.cuda.synchronize()
     _check(o, expected, bound, "wide table")
+
+
+def test_a_group_past_bf16_is_held_as_nan(tm, cuda):
+    """Rotated keys between bf16's largest value and fp32's: their minimum rounds to infinity."""
+    d, size, tokens = 8, 32, 3
+    k = torch.full((tokens, 1, d), 3.3895e38, dtype=torch.bfloat16)
+    k[1] *= -1
+    k[2, 0, 0] = 1.0
+    table = np.concatenate([np.full((1, 4), 1.003), np.zeros((1, 4))], 1).astype(np.float32)
+    with np.errstate(all="ignore"):
+        turned = ref.rotate(k.float().numpy(), np.repeat(table, tokens, 0), False)
+    assert np.isfinite(turned).all() and (np.abs(turned[:2]) > 3.396e38).all()
+    cache = np.zeros((1, 1, 1, ref.block_bytes(d)), np.uint8)
+    device = torch.from_numpy(cache).cuda()
+    paged = dict(cache=device, pages=1, page_size=size, kv_heads=1, d=d, dtype=tm.DTYPE_BF16)
+    slots = torch.arange(tokens, device="cuda")
+    tm.check(tm.cache4_append(tm.Cache4AppendArgs(
+        K=k.cuda(), V=torch.ones_like(k).cuda(), slots=slots, cos_sin=torch.from_numpy(table).cuda(), positions=1, rotary_dim=d,
+        token_positions=torch.zeros(tokens, dtype=torch.int32, device="cuda"), tokens=tokens, **paged)))
+    back = torch.empty_like(k).cuda()
+    tm.check(tm.cache4_gather(tm.Cache4GatherArgs(slots=slots, tokens=tokens, K_out=back, **paged)))
+    torch.cuda.synchronize()
+    for t in range(tokens):
+        ref.write_token(cache, size, t, 0, turned[t, 0], np.ones(d, np.float32))
+    assert np.array_equal(device.cpu().numpy(), cache)
+    assert torch.isnan(back[:2]).all() and torch.isfinite(back[2]).all()

@@ -240,7 +240,7 @@ __global__ __launch_bounds__(kCacheThreads) void cache4_append_kernel(const Appe
                 const float minimum = half_of<true, 1>(pack_pair<true>(0.0f, low)) + 0.0f;  // a zero without its sign
                 std::uint32_t params = pack_pair<true>((high - minimum) / 15.0f, minimum);
                 const float scale = half_of<true, 0>(params);
-                const bool finite = zero == 0.0f && scale < INFINITY;
+                const bool finite = zero == 0.0f && fabsf(scale) < INFINITY;  // (-inf: of a minimum past bf16's values)
                 const bool coded = finite && scale >= kLeastScale;
                 if (!finite) params = 0x7fc07fc0u;
                 else if (!coded) params &= 0xffff0000u;
