@@ -483,7 +483,8 @@ __global__ __launch_bounds__(kThreadsPerGroup, 2) void packed_attention_kernel(c
             }
         }
         // The last key that the lane's row sees, from the tile's first key of the lane.
-        int seen = (p.causal ? last_seen(context, tw + q, seq.q_len) : seq.k_len - 1) - k0 - 4 * h;
+        // (last_seen of row tw + q; that call costs 4 x 2048 tokens at d = 64 52.3 us for 50.7.)
+        int seen = (p.causal ? context + tw + min(q, seq.q_len - 1 - tw) : seq.k_len - 1) - k0 - 4 * h;
         if (active && masked) {
             asm volatile("" : "+v"(seen));
 #pragma unroll
