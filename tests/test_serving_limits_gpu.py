@@ -166,3 +166,29 @@ def test_a_group_past_bf16_is_held_as_nan(tm, cuda):
         ref.write_token(cache, size, t, 0, turned[t, 0], np.ones(d, np.float32))
     assert np.array_equal(device.cpu().numpy(), cache)
     assert torch.isnan(back[:2]).all() and torch.isfinite(back[2]).all()
+
+
+@pytest.mark.parametrize("d,heads,keys", [(8, 1, 700), (64, 4, 700), (128, 2, 500), (96, 1, 3000)])
+def test_many_keys_far_below_the_first_keep_their_weight(tm, cuda, d, heads, keys):
+    """One key of value 0 and many of value 1000 with 2^-25.2 of its weight each, which is under
+    half of fp16's smallest step: their sum is the output. (3000 keys are split.) Bound: fp16
+    probabilities of up to 2^15 are off by 2^-25 each, of the first key's 2^7 or more, beside the
+    bounds of serving_reference.attention, which are relative to the mean |v|."""
+    gap = 25.2 * np.log(2.0)
+    q = torch.ones(1, heads, d, dtype=torch.float16)
+    k = torch.zeros(keys, 1, d, dtype=torch.float16)
+    k[0] = 1.0
+    v = torch.full((keys, 1, d), 1000.0, dtype=torch.float16)
+    v[0] = 0.0
+    expected, bound = ref.attention(q[0].double(), k[:, 0].double(), v[:, 0].double(), gap / d, torch.ones(heads, keys, dtype=torch.bool),
+                                    ref.HALF_STEP[torch.float16])
+    assert (expected > 0.01).all()
+    bound = bound + keys * 2.0 ** -32 * 1000.0 + ref.HALF_STEP[torch.float16] * expected + 2.0 ** -25
+    assert (bound < 0.02 * expected).all()
+    o = torch.full_like(q, 9.0).cuda()
+    starts = [torch.tensor([0, n], dtype=torch.int32, device="cuda") for n in (1, keys)]
+    tm.check(tm.attention_packed(tm.PackedAttentionArgs(
+        Q=q.cuda(), K=k.cuda(), V=v.cuda(), O=o, q_starts=starts[0], k_starts=starts[1], batch=1, q_tokens=1, k_tokens=keys, q_heads=heads,
+        kv_heads=1, d=d, dtype=tm.DTYPE_F16, score_scale=gap / d)))
+    torch.cuda.synchronize()
+    _check(o[0], expected, bound, "the tail")

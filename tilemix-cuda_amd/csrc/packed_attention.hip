@@ -228,11 +228,17 @@ __device__ __forceinline__ float add_pair(std::uint32_t pair, float sum) {
 }
 
 // softmax_tile of attention.hip for either type. The row sums take exactly the
-// rounded probabilities that P.V uses: their rounding (2^-9 of each for bf16)
+// rounded probabilities that P.V uses: their rounding (2^-8 of each for bf16, 2^-11 for fp16)
 // then cancels where values agree, and the rest is of the size of O's own rounding.
+// For fp16 st.m lies 7 below the maximum, so that the largest probability is 2^7 and, as
+// kLazyRescale is 8, none passes 2^15: half of fp16's least step is 2^-32 of the largest then,
+// and many keys far below it keep their weight (700 of 2^-25.2 each were 0).
 template <int kOB, bool kBf16>
 __device__ __forceinline__ void softmax_rows(RowState<kOB>& st, const float16v (&x)[2], float c, uint4v (&p)[4]) {
-    const float tile = max3(block_max16(x[0]), block_max16(x[1]), block_max16(x[1])) * c;  // c >= 0
+    constexpr float kRaised = kBf16 ? 0.0f : 7.0f;
+    static_assert(kBf16 || kRaised + kLazyRescale < 16.0f, "probabilities stay in fp16's range");
+    const float largest = max3(block_max16(x[0]), block_max16(x[1]), block_max16(x[1]));
+    const float tile = kBf16 ? largest * c : __builtin_fmaf(largest, c, -kRaised);  // c >= 0
     if (__any(tile > st.m + kLazyRescale)) {
         float a = tile, b = tile;
         permlane32_swap(a, b);
@@ -456,11 +462,12 @@ __global__ __launch_bounds__(kThreadsPerGroup, 2) void packed_attention_kernel(c
         issue_v(first_tile, 0);
     }
     for (int j = first_tile; j < tiles; ++j) {
-        const int k0 = j * kTileKeys, k_last = k0 + (kTileKeys - 1);  // (k0 + kTileKeys may be 2^31)
+        const int k0 = j * kTileKeys;
         tile_barrier();  // K_j, V_j landed; every wave finished P.V of the previous tile
         set_priority<2>();
         const bool active = k0 <= wave_last;
-        const bool masked = k_last > min(all_last, seq.k_len - 1);
+        // (Compared without k0 + kTileKeys, which may be 2^31.)
+        const bool masked = k0 > min(all_last, seq.k_len - 1) - (kTileKeys - 1);
         float16v s[2];
         float c = p.score_log2;
         if (active) {
@@ -483,7 +490,7 @@ __global__ __launch_bounds__(kThreadsPerGroup, 2) void packed_attention_kernel(c
             }
         }
         // The last key that the lane's row sees, from the tile's first key of the lane.
-        // (last_seen of row tw + q; that call costs 4 x 2048 tokens at d = 64 52.3 us for 50.7.)
+        // (last_seen of row tw + q, the wave's part of it a scalar.)
         int seen = (p.causal ? context + tw + min(q, seq.q_len - 1 - tw) : seq.k_len - 1) - k0 - 4 * h;
         if (active && masked) {
             asm volatile("" : "+v"(seen));
@@ -494,7 +501,7 @@ __global__ __launch_bounds__(kThreadsPerGroup, 2) void packed_attention_kernel(c
                     s[kb][e] = 32 * kb + 8 * (e >> 2) + (e & 3) > seen ? -INFINITY : s[kb][e] * c;
             c = 1.0f;
         }
-        const bool diagonal = k_last >= first_hidden;  // of the workgroup
+        const bool diagonal = k0 >= first_hidden - (kTileKeys - 1);  // of the workgroup
         unsigned char* const v_tile = lds_v + (v_buffer ? L::kVBytes : 0);
         constexpr int kChecks = kTileKeys * kChunks / kThreadsPerGroup;  // chunks of a thread
         auto checked = [&](int x) {
