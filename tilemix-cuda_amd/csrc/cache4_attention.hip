@@ -8,7 +8,7 @@
 // and its bits are the code's, shifted, under a constant exponent - one shift and
 // one and-or for two codes, no subtraction, no scaling. The 16 is taken out by the
 // accumulator's start (-16 sum q) and beside the minimum. q . k is exact but for
-// fp32 sums; of p scale, two bf16 parts (hi + lo, 2^-17 of it) are multiplied, as
+// fp32 sums; of p scale, two bf16 parts (hi + lo, 2^-16 of it) are multiplied, as
 // bf16 holds any scale (fp16 would not).
 //
 // What bounds it is memory: 144 bytes a token and head at d = 128. The cache lies
