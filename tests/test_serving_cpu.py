@@ -263,3 +263,18 @@ def test_rows_of_a_block_table_are_as_far_apart_as_the_call_says(tm, monkeypatch
     assert table((2, 1)) and table((7, 1), table_stride=7) and table((7, 1), batch=1)
     assert not table((7, 1)) and not table((2, 1), table_stride=7) and not table((1, 2)) and not table((14, 2), table_stride=14)
     assert table((1, 5), max_pages=1) and table((5, 5), max_pages=1, table_stride=5) and not table((2,))
+
+
+@pytest.mark.parametrize("kind,rows,heads", [("packed", "q_tokens", 4), ("packed", "k_tokens", 2), ("append", "tokens", 2),
+                                             ("gather", "tokens", 2), ("decode", "batch", 4)])
+def test_strides_whose_reach_passes_63_bits_are_refused(tm, kind, rows, heads):
+    """2^23 rows 2^40 elements apart: their extent is 2^63, which as a signed product looks like
+    none, and heads that lie inside one another's rows like heads that follow one another."""
+    for name in "qo" if heads == 4 else "kv":
+        for head in (1 << 40, 128):
+            options = {rows: (1 << 23) + 1, f"{name}_row_stride": 1 << 40, f"{name}_head_stride": head}
+            assert code(kind, **options) == INVALID, options
+    import torch
+
+    if not torch.cuda.is_available() and (kind != "packed" or rows == "q_tokens"):  # (key rows at most 2^24 apart) a few rows may lie as far apart
+        assert code(kind, **{f"{name}_row_stride": 1 << 40, f"{name}_head_stride": 128}) != INVALID

@@ -29,6 +29,9 @@ inline bool make_rows(Rows& out, const void* data, int tokens, int heads, int d,
     if (reinterpret_cast<std::uintptr_t>(data) % (2 * static_cast<std::size_t>(piece)) != 0) return false;
     if (out.head < 0 || out.row < 0 || out.head > kMost || out.row > kMost || out.head % piece != 0 || out.row % piece != 0)
         return false;
+    // No memory holds a tensor that reaches further; strided_heads_ok's products fit 63 bits then.
+    constexpr std::int64_t kReach = std::int64_t{1} << 48;
+    if (out.row > kReach / std::max(tokens, 1) || out.head > kReach / heads) return false;
     return strided_heads_ok(heads, std::max(tokens, 1), d, out.head, out.row);
 }
 
