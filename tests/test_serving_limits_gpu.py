@@ -192,3 +192,25 @@ def test_many_keys_far_below_the_first_keep_their_weight(tm, cuda, d, heads, key
         kv_heads=1, d=d, dtype=tm.DTYPE_F16, score_scale=gap / d)))
     torch.cuda.synchronize()
     _check(o[0], expected, bound, "the tail")
+
+
+@pytest.mark.parametrize("dtype,below", [("f16", 20.7), ("f16", 25.2), ("f16", 30.5), ("bf16", 25.2)])
+def test_values_that_agree_come_out_as_they_are(tm, cuda, dtype, below):
+    """The row sums take the probabilities that P.V uses, also those below fp16's normal numbers:
+    of 60000 keys `below` bits under the first one, which weigh up to 3 % together, the average of
+    ones is 1. (As many rows as not to be split.) O is summed in steps of 8 keys or more and the row
+    sum in one per tile and lane, each off by up to half an fp32 step of a sum that hardly grows:
+    (keys / 8 + keys / 64 + 64) 2^-24 = 5.1e-4 in all, and the output's half step; a sum that had
+    left out the keys 25.2 bits under the first would be 1.6e-3 off."""
+    d, heads, rows, keys = 8, 8, 4160, 60000
+    q = torch.ones(rows, heads, d, dtype=DT[dtype], device="cuda")
+    k = torch.zeros(keys, heads, d, dtype=DT[dtype], device="cuda")
+    k[0] = 1.0
+    v = torch.ones_like(k)
+    o = torch.full_like(q, 9.0)
+    starts = [torch.tensor([0, n], dtype=torch.int32, device="cuda") for n in (rows, keys)]
+    tm.check(tm.attention_packed(tm.PackedAttentionArgs(
+        Q=q, K=k, V=v, O=o, q_starts=starts[0], k_starts=starts[1], batch=1, q_tokens=rows, k_tokens=keys, q_heads=heads, kv_heads=heads,
+        d=d, dtype=_code(tm, dtype), score_scale=float(below * np.log(2.0) / d), causal=False)))
+    torch.cuda.synchronize()
+    assert float((o.double() - 1.0).abs().max()) <= (keys / 8 + keys / 64 + 64) * ref.FP32 + ref.HALF_STEP[DT[dtype]]
