@@ -26,7 +26,7 @@
 // head: those go to the workspace, where the workgroup that arrives last merges them in order.
 //
 // Measured: 64 sequences of 1 to 16384 tokens, 32 query and 8 key heads x 128: 93 us, 4.5 TB/s;
-// 2 of 32768 tokens, 16 heads: 36 us, 4.2 TB/s; 64 of 8192 tokens, 8 key heads, 5.2 TB/s. A
+// 2 of 32768 tokens, 16 heads: 35 to 39 us, 3.9 to 4.3 TB/s; 64 of 8192 tokens, 8 key heads, 5.2 TB/s. A
 // range's start and end take about 6 us. One sequence of 1003
 // tokens, 4 key heads x 64: 9.7 us.
 
@@ -192,7 +192,9 @@ __device__ __forceinline__ bool first_segment(const DecodeParams& p, int range, 
     // Sequences that are all alike: whole ranges for each sequence and head, or whole sequences for
     // a range, so that no range ends inside one, if that is hardly more for each or leaves at
     // least two of three workgroups (2 sequences of 32768 tokens, 16 heads: 40.7 us cut anywhere,
-    // 35.4 so; 64 of 2048, 8 heads: 37.8 and 33.2; 128, 8 heads, of 1024: 43.0 and 37.7).
+    // 35.4 so; 64 of 2048, 8 heads: 37.8 and 33.2; 128, 8 heads, of 1024: 43.0 and 37.7). One a
+    // few blocks shorter than the others, or empty, has them cut anywhere: 32768 and 32700 tokens
+    // 37.7 us for 34.6, 128 of 985 to 1024 42.1 for 35.8.
     if (alike && items <= ranges) {
         const unsigned each = ranges / items;
         const int length = max(static_cast<int>((sequence0 + each - 1) / each), least);

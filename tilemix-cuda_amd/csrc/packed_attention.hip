@@ -24,7 +24,7 @@
 // Long walks are bound by the matrix unit at the power limit's clock beside the softmax's
 // vector work: 16384 tokens, 32 heads (8 key heads) x 128, causal, bf16: 2.0 ms, 1.05
 // PFLOP/s, matrix unit busy 57 % of cycles. Short ones by a block's start and end, about
-// 10 us (queries, first tiles, O): 16 x 1024 tokens 190 to 235 us, 0.6 to 0.7 PFLOP/s;
+// 10 us (queries, first tiles, O): 16 x 1024 tokens 182 to 235 us, 0.6 to 0.75 PFLOP/s;
 // one of 250 tokens 6 us.
 
 #include "attention_tiles.h"
@@ -134,7 +134,8 @@ struct Work {
 // Up to 64 sequences, one a lane: in order where all blocks start at once, else blocks of more
 // key tiles first (the last to start are the shortest; a long walk that starts last would run
 // alone), found by a search over tile counts. More sequences keep their order, as
-// every step of that search would read all of their lengths (1000 sequences of 50 tokens, 32 heads: 707 us, 150 so): sequence b's blocks
+// every step of that search would read all of their lengths (1000 sequences of 50 tokens, 32 heads: 707 us, 150 so;
+// what the order costs: 100 of 200 tokens and one of 8192, 612 to 622 us with the long one first, 624 to 626 last): sequence b's blocks
 // have the numbers from floor(start / tokens of a block) + b on, which leaves room for
 // all of them, and is found by a search over the starts. Numbers left over have no work.
 template <bool kSplit>
@@ -321,7 +322,7 @@ __global__ __launch_bounds__(kThreadsPerGroup, 2) void packed_attention_kernel(c
     constexpr int kQuads = 4 * kOB;
     // kInTurn: O of the ranges so far, [quad][thread]. (Dynamic, as an array of known size would
     // have the compiler allocate accumulation registers for one workgroup a CU, which the softmax
-    // pays for: 2 x 512 tokens after 7680 keys 245 us, 195 so; 168 in one piece.)
+    // pays for: 2 x 512 tokens after 7680 keys 245 us, when 195 so; now 169, in one piece 160.)
     extern __shared__ float4v lds_merged[];
     unsigned char* const lds_k = smem;
     unsigned char* const lds_v = smem + L::kKBytes;
